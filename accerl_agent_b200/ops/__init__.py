@@ -8,7 +8,8 @@ weights keep the HF ``[out_features, in_features]`` layout.
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Tuple
+from dataclasses import dataclass
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 
@@ -86,6 +87,11 @@ __all__ = [
     "kv_cache_write",
     "qkv_rope_cache",
     "sample",
+    "Int8Rows",
+    "quantize_rows",
+    "rmsnorm_quantize",
+    "swiglu_quantize",
+    "linear_int8",
     "workspace",
 ]
 
@@ -312,6 +318,149 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, grad: torch.Tensor
         return grad
     grad.index_add_(0, ids.reshape(-1), dout.float())
     return grad
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit linear layers
+# ------------------------------------------------------------------------------------------------
+INT8_MAX_K = 133144  # 2^31 / 127^2: longer rows could overflow the 32-bit integer accumulators
+
+
+@dataclass
+class Int8Rows:
+    """Rows in 8-bit integers with one scale each: row ``i`` stands for ``scale[i] * q[i, :k]``.
+
+    ``q`` int8 [rows, k rounded up to 16] (zeros behind ``k``), ``scale`` fp32 [rows]. Activations (a row
+    per token) and weights (a row per output channel) are both kept this way."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.q.shape[0], self.k
+
+    def dequantize(self) -> torch.Tensor:
+        """The fp32 values the rows stand for, [rows, k]."""
+        return self.q[:, : self.k].float() * self.scale.unsqueeze(1)
+
+
+def _int8_rows(rows: int, k: int, device: torch.device, out: Optional[Int8Rows]) -> Int8Rows:
+    kp = (k + 15) // 16 * 16
+    if out is None:
+        return Int8Rows(torch.empty(rows, kp, dtype=torch.int8, device=device),
+                        torch.empty(rows, dtype=torch.float32, device=device), k)
+    if (out.k != k or tuple(out.q.shape) != (rows, kp) or out.scale.numel() != rows or out.q.device != device
+            or out.scale.device != device or out.q.dtype != torch.int8 or out.scale.dtype != torch.float32):
+        raise ValueError(f"out does not hold {rows} x {k} int8 rows on {device}")
+    return out
+
+
+def _check_rows(name: str, x: torch.Tensor, dtypes) -> None:
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"{name} must be [rows, features], got {tuple(x.shape)}")
+    if x.is_cuda and x.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d).split('.')[-1] for d in dtypes)}, got {x.dtype}")
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def quantize_rows(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
+    """``x`` [rows, K] (bf16 or fp16; on the CPU any float type) in 8 bits, per row: ``a = max |x|``,
+    ``scale = a / 127``, ``q = round(127 x / a)``, ties to even, decided exactly. A row of zeros has scale
+    0; a row with an infinity or NaN has scale NaN and zeros, so every product with it is NaN.
+
+    Rows may be strided; sizes and strides that are multiples of 8 take 16-byte accesses."""
+    _check_rows("x", x, (torch.bfloat16, torch.float16))
+    out = _int8_rows(x.shape[0], x.shape[1], x.device, out)
+    if x.is_cuda:
+        native().quantize_rows(x, 0, None, 0.0, out.q, out.scale)
+    else:
+        reference.quantize_rows(x, out.q, out.scale)
+    return out
+
+
+def rmsnorm_quantize(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[Int8Rows] = None) -> Int8Rows:
+    """``quantize_rows(rmsnorm(x, w, eps)[0])`` in one pass over ``x`` (bf16 [rows, K]; on the GPU K is a
+    multiple of 8 up to 32768). The normalised rows are rounded to bf16 as ``rmsnorm`` rounds them."""
+    _check_rows("x", x, (torch.bfloat16,))
+    if w.numel() != x.shape[1] or w.device != x.device or (x.is_cuda and w.dtype != x.dtype):
+        raise ValueError("the norm weight must be [K], of x's type and on x's device")
+    out = _int8_rows(x.shape[0], x.shape[1], x.device, out)
+    if x.is_cuda:
+        if x.shape[1] % 8 or x.shape[1] > 32768 or x.stride(0) % 8 or x.data_ptr() % 16 or w.data_ptr() % 16:
+            raise ValueError("rmsnorm_quantize needs rows of a multiple of 8 (at most 32768) elements, aligned to 16 bytes")
+        native().quantize_rows(x, 1, w.contiguous(), eps, out.q, out.scale)
+    else:
+        reference.quantize_rows(reference.rmsnorm(x, w, eps)[0], out.q, out.scale)
+    return out
+
+
+def swiglu_quantize(gu: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
+    """``quantize_rows(swiglu(gu))`` in one pass over ``gu`` = gate | up (bf16 [rows, 2K]; on the GPU K is a
+    multiple of 8 up to 32768). Same bits as the two calls."""
+    _check_rows("gu", gu, (torch.bfloat16,))
+    if gu.shape[1] % 2:
+        raise ValueError("gu must be [rows, 2K]")
+    k = gu.shape[1] // 2
+    out = _int8_rows(gu.shape[0], k, gu.device, out)
+    if gu.is_cuda:
+        if k % 8 or k > 32768 or gu.stride(0) % 8 or gu.data_ptr() % 16:
+            raise ValueError("swiglu_quantize needs K a multiple of 8 (at most 32768) and rows aligned to 16 bytes")
+        native().quantize_rows(gu, 2, None, 0.0, out.q, out.scale)
+    else:
+        reference.quantize_rows(reference.swiglu(gu), out.q, out.scale)
+    return out
+
+
+def linear_int8(x: Union[torch.Tensor, Int8Rows], w: Int8Rows, bias: Optional[torch.Tensor] = None,
+                residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``y = x w^T (+bias) (+residual)`` with 8-bit operands: ``y[t, n] = x.scale[t] * w.scale[n] *
+    sum_k x.q[t, k] w.q[n, k]``. The integer sum is exact, the rest is fp32, rounded once.
+
+    ``x``: int8 rows, or bf16 / fp16 activations [T, in], which are quantised first. ``w``: int8 rows of
+    the weight [out, in] (``quantize_rows(weight)``). The result is ``out`` (rows may be strided, last
+    dimension contiguous), else a tensor of ``out_dtype`` (default: x's own type, bf16 for int8 rows);
+    bf16, fp16 or fp32. ``bias`` [out] and ``residual`` [T, out] are of one such type; ``residual`` may be
+    ``out`` itself. ``in`` is at most ``INT8_MAX_K``."""
+    if not isinstance(w, Int8Rows):
+        raise ValueError("w must be Int8Rows: quantize_rows(weight)")
+    if not isinstance(x, Int8Rows):
+        out_dtype = out_dtype or x.dtype
+        if x.dim() == 2 and x.shape[1] != w.k:
+            raise ValueError(f"inner dimensions differ ({x.shape[1]} vs {w.k})")
+        x = quantize_rows(x)
+    M, N, K = x.q.shape[0], w.q.shape[0], w.k
+    dev = w.q.device
+    if x.k != K:
+        raise ValueError(f"inner dimensions differ ({x.k} vs {K})")
+    if K > INT8_MAX_K:
+        raise ValueError(f"in must be at most {INT8_MAX_K}, got {K}")
+    floats = (torch.bfloat16, torch.float16, torch.float32)
+    if out is None:
+        out_dtype = out_dtype or torch.bfloat16
+        if out_dtype not in floats:
+            raise ValueError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    elif tuple(out.shape) != (M, N) or out.dtype not in floats or (N > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be bf16, fp16 or fp32 [{M}, {N}] with a contiguous last dimension")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in floats or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous bf16, fp16 or fp32 [{N}]")
+    if residual is not None and (tuple(residual.shape) != (M, N) or residual.dtype not in floats
+                                 or (N > 1 and residual.stride(1) != 1)):
+        raise ValueError(f"residual must be bf16, fp16 or fp32 [{M}, {N}] with a contiguous last dimension")
+    if bias is not None and residual is not None and bias.dtype != residual.dtype:
+        raise ValueError("bias and residual must be of one type")
+    for t in (x.q, x.scale, w.scale, out, bias, residual):
+        if t is not None and t.device != dev:
+            raise ValueError(f"every tensor must be on the weight's device {dev}, got one on {t.device}")
+    if dev.type == "cuda":
+        native().gemm_int8(x.q, x.scale, w.q, w.scale, K, bias, residual, out, status_tensor(dev))
+    else:
+        out.copy_(reference.linear_int8(x.q, x.scale, w.q, w.scale, bias, residual))
+    return out
 
 
 # ------------------------------------------------------------------------------------------------

@@ -70,6 +70,30 @@ def swiglu_backward(dh: torch.Tensor, gu: torch.Tensor) -> torch.Tensor:
     return torch.cat([dhf * u * dact, dhf * act], dim=-1).to(gu.dtype)
 
 
+def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """Rows of ``x`` [rows, K] in 8 bits into ``q`` int8 [rows, >= K] (zeros behind K) and ``scale`` [rows]:
+    a = max |x|, scale = a / 127, q = round(127 x / a) with ties to even (the quotient in 64 bits, where 127 x
+    is exact). Rows of zeros: scale 0. Rows with an infinity or NaN: scale NaN, q = 0."""
+    xf = x.float()
+    a = xf.abs().amax(1, keepdim=True)
+    ok = torch.isfinite(a)
+    r = torch.round(127.0 * xf.double() / a.double())
+    q.zero_()
+    q[:, : x.shape[1]] = torch.where(ok & (a > 0), r, torch.zeros_like(r)).to(torch.int8)
+    scale.copy_(torch.where(ok, a / 127.0, torch.full_like(a, float("nan"))).squeeze(1))
+
+
+def linear_int8(qx, sx, qw, sw, bias=None, residual=None) -> torch.Tensor:
+    """fp32 ``sx sw (qx qw^T) (+ bias) (+ residual)``; the integer sum in 64-bit floats, where it is exact."""
+    acc = qx.double() @ qw.double().t()
+    y = acc.float() * (sx.unsqueeze(1) * sw.unsqueeze(0))
+    if bias is not None:
+        y = y + bias.float()
+    if residual is not None:
+        y = y + residual.float()
+    return y
+
+
 def attention_varlen(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, causal: bool = True
 ) -> Tuple[torch.Tensor, torch.Tensor]:

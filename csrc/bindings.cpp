@@ -122,6 +122,11 @@ int accerl_sample_logits(const void* logits, long long ld, int rows, int V, cons
                          const int* top_k, const float* top_p, const unsigned long long* seeds,
                          const long long* offsets, long long* out_tokens, float* out_logprobs, float* part,
                          int num_chunks, cudaStream_t s);
+int accerl_quantize_rows(const void* x, long long ldx, int half, int pre, const void* w, float eps, void* q,
+                         float* scale, long long rows, int K, cudaStream_t s);
+int accerl_gemm_int8(const void* qx, const float* sx, const void* qw, const float* sw, int M, int N, int K,
+                     const void* bias, const void* residual, long long ldr, int in_type, void* out, long long ldo,
+                     int out_type, int* status, cudaStream_t stream);
 }
 
 namespace {
@@ -772,6 +777,76 @@ void sample_logits(const at::Tensor& logits, const at::Tensor& temperature, cons
         "sample_logits");
 }
 
+// x [rows, K] (pre 0: as it is, 1: RMSNorm with weight w, 2: SwiGLU of gate | up [rows, 2K]) -> int8 rows
+// q [rows, K rounded up to 16] and scale [rows].
+void quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w, double eps, at::Tensor& q,
+                   at::Tensor& scale) {
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
+  CHECK_CUDA(x);
+  CHECK_CUDA(q);
+  CHECK_CUDA(scale);
+  CHECK_F32(scale);
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "quantize_rows: bf16 or fp16 rows");
+  const int64_t K = pre == 2 ? x.size(1) / 2 : x.size(1);
+  TORCH_CHECK(q.scalar_type() == at::kChar && q.is_contiguous() && q.size(0) == x.size(0) &&
+                  q.size(1) == (K + 15) / 16 * 16,
+              "quantize_rows: q must be int8 [rows, K rounded up to 16]");
+  TORCH_CHECK(scale.is_contiguous() && scale.numel() == x.size(0), "quantize_rows: scale [rows]");
+  if (pre == 1) {
+    TORCH_CHECK(w.has_value() && w->is_cuda() && w->numel() == K && w->is_contiguous(), "quantize_rows: norm weight [K]");
+    CHECK_BF16(*w);
+  }
+  check(accerl_quantize_rows(x.data_ptr(), ld_of(x), x.scalar_type() == at::kHalf, static_cast<int>(pre), opt_ptr(w),
+                             static_cast<float>(eps), q.data_ptr(), scale.data_ptr<float>(), x.size(0),
+                             static_cast<int>(K), cur_stream()),
+        "quantize_rows");
+}
+
+int float_type_id(const at::Tensor& t) {
+  if (t.scalar_type() == at::kBFloat16) return 0;
+  if (t.scalar_type() == at::kHalf) return 1;
+  TORCH_CHECK(t.scalar_type() == at::kFloat, "expected bf16, fp16 or f32");
+  return 2;
+}
+
+// out [M, N] = sx sw (qx qw^T) (+ bias) (+ residual); bias and residual share one type
+void gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
+               const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, at::Tensor& out,
+               const c10::optional<at::Tensor>& status) {
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(qx));
+  CHECK_CUDA(qx);
+  CHECK_CUDA(qw);
+  CHECK_CUDA(out);
+  CHECK_F32(sx);
+  CHECK_F32(sw);
+  const int64_t M = qx.size(0), N = qw.size(0), Kp = (K + 15) / 16 * 16;
+  TORCH_CHECK(qx.scalar_type() == at::kChar && qw.scalar_type() == at::kChar, "gemm_int8: int8 operands");
+  TORCH_CHECK(qx.is_contiguous() && qw.is_contiguous() && qx.size(1) == Kp && qw.size(1) == Kp,
+              "gemm_int8: operands must be contiguous [rows, K rounded up to 16]");
+  TORCH_CHECK(sx.is_cuda() && sw.is_cuda() && sx.is_contiguous() && sw.is_contiguous() && sx.numel() == M &&
+                  sw.numel() == N,
+              "gemm_int8: one scale per row");
+  TORCH_CHECK(out.size(0) == M && out.size(1) == N, "gemm_int8: output shape mismatch");
+  int in_type = float_type_id(out);
+  long long ldr = 0;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->is_cuda() && residual->size(0) == M && residual->size(1) == N,
+                "gemm_int8: residual shape mismatch");
+    in_type = float_type_id(*residual);
+    ldr = ld_of(*residual);
+  }
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->is_cuda() && bias->numel() == N && bias->is_contiguous(), "gemm_int8: bias must be contiguous [N]");
+    TORCH_CHECK(!residual.has_value() || float_type_id(*bias) == in_type, "gemm_int8: bias and residual types differ");
+    in_type = float_type_id(*bias);
+  }
+  check(accerl_gemm_int8(qx.data_ptr(), sx.data_ptr<float>(), qw.data_ptr(), sw.data_ptr<float>(),
+                         static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), opt_ptr(bias),
+                         opt_ptr(residual), ldr, in_type, out.data_ptr(), ld_of(out), float_type_id(out),
+                         status_ptr(status), cur_stream()),
+        "gemm_int8");
+}
+
 }  // namespace
 
 // Debug-checks build records, one (code, index) pair per kernel source file (code 0: no failed check).
@@ -890,6 +965,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_decode", &paged_decode);
   m.def("kv_cache_write", &kv_cache_write);
   m.def("sample_logits", &sample_logits);
+  m.def("quantize_rows", &quantize_rows, "rows to int8 with a scale each, optionally behind RMSNorm or SwiGLU");
+  m.def("gemm_int8", &gemm_int8, "tcgen05 int8 GEMM with token and channel scales");
   m.def("enable_peer_access", &enable_peer_access);
   m.def("rs_sumsq", &rs_sumsq);
   m.def("adamw_push", &adamw_push);
