@@ -87,6 +87,7 @@ __all__ = [
     "kv_cache_write",
     "qkv_rope_cache",
     "sample",
+    "sample_inverse_cdf",
     "Int8Rows",
     "quantize_rows",
     "rmsnorm_quantize",
@@ -830,3 +831,45 @@ def sample(logits, temperature, seeds, offsets, num_chunks: int = 16, generator=
             LAUNCHES[0] += 1
         return tokens, lps
     return reference.sample_reference(logits, temperature, generator, top_k, top_p)
+
+
+SAMPLE_MAX_VOCAB = 524208  # what one cluster's 16-bit counters can hold
+
+
+def sample_inverse_cdf(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
+                       top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                       min_p: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Sample one token per row of ``logits`` [rows, V] (bf16 or fp16 on the GPU) from the given numbers
+    ``u`` [rows] in [0, 1): the same inputs always give the same tokens, whatever else is in the batch.
+
+    With the row's tokens in order of descending logit (ties: lowest index first), the candidates are the
+    first ``top_k`` of them (int32 [rows], <= 0: off), of these the ones whose weight
+    ``w = exp((x - max) / temperature)`` is at least ``min_p`` (float32 [rows], 0: off), and of these the
+    ones whose preceding weights sum to less than ``top_p`` (float32 [rows], >= 1: off) times their sum;
+    the first candidate always stays. The token is the first one whose cumulative weight exceeds ``u``
+    times the candidates' sum. ``temperature`` (float32 [rows]) <= 0 takes the largest logit. Weights and
+    sums are 64-bit.
+
+    Logits of -inf and NaN are never chosen, -0 ties with 0, and +inf shares the mass with its equals. A
+    row without any other logit gives token 0 with log-probability -inf. ``u`` outside [0, 1) counts as
+    the nearest number inside, NaN as 0; a NaN temperature as 0, a NaN ``top_p`` or ``min_p`` as off.
+    Returns (tokens int64 [rows], log-probability float32 [rows] of each under softmax(logits))."""
+    if logits.dim() != 2 or not 0 < logits.shape[1] <= SAMPLE_MAX_VOCAB:
+        raise ValueError(f"logits must be [rows, 1..{SAMPLE_MAX_VOCAB}], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("the last dimension of logits must be contiguous")
+    if logits.is_cuda and logits.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"logits must be bf16 or fp16, got {logits.dtype}")
+    for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
+                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32)):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous()
+                              or t.device != logits.device):
+            raise ValueError(f"{name} must be contiguous {dtype} [{rows}] on {logits.device}")
+    if not logits.is_cuda:
+        return reference.sample_inverse_cdf(logits, u, temperature, top_k, top_p, min_p)
+    tokens = torch.empty(rows, dtype=torch.long, device=logits.device)
+    lps = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    native().sample_counts(logits, u, temperature, top_k, top_p, min_p, tokens, lps)
+    return tokens, lps

@@ -210,5 +210,43 @@ def sample_reference(logits: torch.Tensor, temperature: torch.Tensor, generator:
     return tokens, logp.gather(1, tokens.view(-1, 1)).squeeze(1)
 
 
+def sample_inverse_cdf(logits, u, temperature, top_k=None, top_p=None, min_p=None):
+    """Row by row in 64 bits: sort, cut (top_k, min_p, top_p), first cumulative weight above u times the sum."""
+    rows = logits.shape[0]
+    tokens = torch.zeros(rows, dtype=torch.long, device=logits.device)
+    lps = torch.full((rows,), float("-inf"), dtype=torch.float32, device=logits.device)
+    for i in range(rows):
+        x = logits[i].double()
+        ids = torch.nonzero(x > float("-inf")).squeeze(1)  # NaN and -inf compare false
+        if ids.numel() == 0:
+            continue
+        vals, order = torch.sort(x[ids], descending=True, stable=True)
+        ids = ids[order]
+        first = vals == vals[0]
+        gap = torch.where(first, torch.zeros_like(vals), vals - vals[0])  # inf - inf counts as 0
+        t = float(temperature[i])
+        w = torch.where(first, torch.ones_like(gap), torch.exp(gap / t)) if t > 0 else first.double()
+        w = torch.nan_to_num(w)  # -inf / inf: no weight
+        n = w.numel() if t > 0 else 1
+        k = int(top_k[i]) if top_k is not None else 0
+        if 0 < k < n:
+            n = k
+        m = float(min_p[i]) if min_p is not None else 0.0
+        if m > 0:
+            n = min(n, max(1, int((w >= m).sum())))
+        cum = torch.cumsum(w[:n], 0)
+        p = float(top_p[i]) if top_p is not None else 1.0
+        if p < 1.0 and t > 0:
+            n = int(torch.nonzero(cum >= max(p, 0.0) * cum[-1])[0]) + 1
+            cum = cum[:n]
+        r = float(u[i])
+        r = min(max(r, 0.0), 1.0 - 2.0 ** -53) if r == r else 0.0
+        above = torch.nonzero(cum > r * cum[-1])
+        at = int(above[0]) if above.numel() else int(torch.nonzero(w[:n] > 0)[-1])
+        tokens[i] = ids[at]
+        lps[i] = (gap[at] - torch.exp(gap).sum().log()).float()
+    return tokens, lps
+
+
 def default_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)

@@ -122,6 +122,9 @@ int accerl_sample_logits(const void* logits, long long ld, int rows, int V, cons
                          const int* top_k, const float* top_p, const unsigned long long* seeds,
                          const long long* offsets, long long* out_tokens, float* out_logprobs, float* part,
                          int num_chunks, cudaStream_t s);
+int accerl_sample_counts(const void* logits, long long ld, int half, int rows, int V, const float* u,
+                         const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                         long long* tokens, float* logprobs, cudaStream_t s);
 int accerl_quantize_rows(const void* x, long long ldx, int half, int pre, const void* w, float eps, void* q,
                          float* scale, long long rows, int K, cudaStream_t s);
 int accerl_gemm_int8(const void* qx, const float* sx, const void* qw, const float* sw, int M, int N, int K,
@@ -777,6 +780,35 @@ void sample_logits(const at::Tensor& logits, const at::Tensor& temperature, cons
         "sample_logits");
 }
 
+// One token per row of logits [rows, V] from the uniform numbers u [rows].
+void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tensor& temperature,
+                   const c10::optional<at::Tensor>& top_k, const c10::optional<at::Tensor>& top_p,
+                   const c10::optional<at::Tensor>& min_p, at::Tensor& out_tokens, at::Tensor& out_logprobs) {
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(logits));
+  const int64_t rows = logits.size(0);
+  CHECK_CUDA(logits);
+  TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf, "logits must be bf16 or fp16");
+  auto f32 = [&](const at::Tensor& t, const char* name) -> const float* {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == rows, name,
+                " must be contiguous float32 [rows]");
+    return t.data_ptr<float>();
+  };
+  const int* tk = nullptr;
+  if (top_k.has_value()) {
+    TORCH_CHECK(top_k->is_cuda() && top_k->scalar_type() == at::kInt && top_k->is_contiguous() && top_k->numel() == rows,
+                "top_k must be contiguous int32 [rows]");
+    tk = top_k->data_ptr<int>();
+  }
+  CHECK_I64(out_tokens);
+  check(accerl_sample_counts(logits.data_ptr(), ld_of(logits), logits.scalar_type() == at::kHalf,
+                             static_cast<int>(rows), static_cast<int>(logits.size(1)), f32(u, "u"),
+                             f32(temperature, "temperature"), tk, top_p.has_value() ? f32(*top_p, "top_p") : nullptr,
+                             min_p.has_value() ? f32(*min_p, "min_p") : nullptr,
+                             reinterpret_cast<long long*>(out_tokens.data_ptr<int64_t>()),
+                             out_logprobs.data_ptr<float>(), cur_stream()),
+        "sample_counts");
+}
+
 // x [rows, K] (pre 0: as it is, 1: RMSNorm with weight w, 2: SwiGLU of gate | up [rows, 2K]) -> int8 rows
 // q [rows, K rounded up to 16] and scale [rows].
 void quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w, double eps, at::Tensor& q,
@@ -965,6 +997,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_decode", &paged_decode);
   m.def("kv_cache_write", &kv_cache_write);
   m.def("sample_logits", &sample_logits);
+  m.def("sample_counts", &sample_counts, "one token per row from given uniform numbers");
   m.def("quantize_rows", &quantize_rows, "rows to int8 with a scale each, optionally behind RMSNorm or SwiGLU");
   m.def("gemm_int8", &gemm_int8, "tcgen05 int8 GEMM with token and channel scales");
   m.def("enable_peer_access", &enable_peer_access);
