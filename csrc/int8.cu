@@ -229,7 +229,6 @@ ACCERL_DEVINL void umma_s8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint
 
 constexpr int kI8BK = 128;         // elements (= bytes) of K per stage: one 128-byte swizzled row
 constexpr int kI8Rows = 128;       // weight rows per tile
-constexpr int kI8MaxTokens = 256;  // tokens per tile
 constexpr int kI8Threads = 192;
 
 enum OutType : int { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2 };
@@ -245,10 +244,20 @@ struct Int8Params {
   long long ldo;
   int out_type;  // of out; bias and residual are in_type
   int in_type;
-  int bt;      // tokens per tile
-  int stages;
+  int bt, stages;                  // few tokens: tokens per tile, ring size
+  int tiles_m, tiles_n, group_m;   // many tokens: the tile grid
   int* status;
 };
+
+ACCERL_DEVINL int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+ACCERL_DEVINL uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 ACCERL_DEVINL float load_as_float(const void* p, long long i, int type) {
   if (type == kOutBf16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
@@ -261,21 +270,26 @@ ACCERL_DEVINL void store_from_float(void* p, long long i, int type, float v) {
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
-// One tile of 128 output channels x bt tokens per CTA: the weight rows are the MMA's 128 rows, so a decode
-// batch of few tokens wastes no tensor rows and streams the weight once.
+// Few tokens: one tile of 128 output channels x bt tokens per cluster of CTAs. The weight rows are the MMA's
+// 128 rows, so a decode batch of few tokens wastes no tensor rows and streams the weight once. The CTAs of a
+// cluster split K (there are only N / 128 tiles to spread over 148 SMs): each leaves its integer partial in its
+// shared memory, and each sums and finishes its share of the tokens over the cluster. Integer sums have no
+// order, so the split changes no bit.
 //   warp 0: TMA producer into a ring of stages;  warp 1: TMEM and MMA issue;  warps 2-5: epilogue (one
 //   TMEM lane = one output channel per thread; the 32 lanes of a warp store 32 neighbouring channels).
-__global__ void __launch_bounds__(kI8Threads) gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW,
-                                                               const __grid_constant__ CUtensorMap tmX,
-                                                               const Int8Params p) {
+__global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __grid_constant__ CUtensorMap tmW,
+                                                                      const __grid_constant__ CUtensorMap tmX,
+                                                                      const Int8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[16], empty[16], done;
   __shared__ uint32_t tmem_slot;
-  __shared__ float sx_s[kI8MaxTokens];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * kI8Rows, t0 = blockIdx.y * p.bt;
-  const int kbs = (p.K + kI8BK - 1) / kI8BK;
+  const int split = blockIdx.z, splits = gridDim.z;
+  const int kbs_all = (p.K + kI8BK - 1) / kI8BK;
+  const int kb_first = static_cast<int>(static_cast<long long>(kbs_all) * split / splits);
+  const int kbs = static_cast<int>(static_cast<long long>(kbs_all) * (split + 1) / splits) - kb_first;
   const uint32_t stage_bytes = (kI8Rows + p.bt) * kI8BK;
   uint32_t cols = 32;
   while (cols < static_cast<uint32_t>(p.bt)) cols <<= 1;
@@ -292,8 +306,6 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_kernel(const __grid_cons
     prefetch_tmap(&tmX);
   }
   if (warp == 1) tmem_alloc(&tmem_slot, cols);
-  if (warp >= 2)
-    for (int i = threadIdx.x - 64; i < p.bt; i += 128) sx_s[i] = t0 + i < p.M ? p.sx[t0 + i] : 0.f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -310,8 +322,8 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_kernel(const __grid_cons
           break;
         }
         mbar_arrive_expect_tx(&full[s], stage_bytes);
-        tma_load_2d(smem + s * stage_bytes, &tmW, &full[s], kb * kI8BK, n0);
-        tma_load_2d(smem + s * stage_bytes + kI8Rows * kI8BK, &tmX, &full[s], kb * kI8BK, t0);
+        tma_load_2d(smem + s * stage_bytes, &tmW, &full[s], (kb_first + kb) * kI8BK, n0);
+        tma_load_2d(smem + s * stage_bytes + kI8Rows * kI8BK, &tmX, &full[s], (kb_first + kb) * kI8BK, t0);
         ++issued;
       }
       // never leave a copy in flight into the shared memory of a finished CTA
@@ -340,38 +352,348 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_kernel(const __grid_cons
       }
       if (ok) umma_commit(&done);
     }
-  } else {
-    const int quarter = warp & 3;  // TMEM lanes this warp may read
-    const int n = n0 + quarter * 32 + lane;
-    if (mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue)) {
-      tc_fence_after();
-      const bool n_ok = n < p.N;
-      const float sw = n_ok ? p.sw[n] : 0.f;
-      const float b = (n_ok && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
+  }
+  // this CTA's share of the tokens of the tile
+  const int share = (p.bt + splits - 1) / splits;
+  const int c_lo = split * share, c_hi = min(min(p.bt, p.M - t0), c_lo + share);
+  const int quarter = warp & 3;  // TMEM lanes this warp may read
+  const int n = n0 + quarter * 32 + lane;
+  const bool n_ok = warp >= 2 && n < p.N;
+  const float sw = n_ok ? p.sw[n] : 0.f;
+  const float b = (n_ok && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
+  auto finish = [&](int c, int acc) {
+    const long long t = t0 + c;
+    float y = static_cast<float>(acc) * (__ldg(p.sx + t) * sw) + b;
+    if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
+    store_from_float(p.out, t * p.ldo + n, p.out_type, y);
+  };
+  bool ok = false;
+  if (warp >= 2) {
+    ok = mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue);
+    tc_fence_after();
+    const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16);
+    if (splits == 1) {
+      if (ok) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < p.bt && t0 + c0 < p.M; c0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(tbase + (static_cast<uint32_t>(quarter * 32) << 16) + c0, v);
-        tmem_wait_ld();
-        if (n_ok) {
+        for (int c0 = 0; c0 < c_hi; c0 += 16) {
+          uint32_t v[16];
+          tmem_ld16(t_row + c0, v);
+          tmem_wait_ld();
+          if (n_ok) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const long long t = t0 + c0 + i;
-            if (t < p.M) {
-              float y = static_cast<float>(static_cast<int>(v[i])) * (sx_s[c0 + i] * sw) + b;
-              if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
-              store_from_float(p.out, t * p.ldo + n, p.out_type, y);
-            }
+            for (int i = 0; i < 16; ++i)
+              if (c0 + i < c_hi) finish(c0 + i, static_cast<int>(v[i]));
           }
         }
       }
-      tc_fence_before();
+    } else if (ok) {
+      // every MMA of this CTA has read its stages: their memory takes the partial, [token][channel]
+      int* part = reinterpret_cast<int*>(smem) + quarter * 32 + lane;
+#pragma unroll 1
+      for (int c0 = 0; c0 < min(p.bt, p.M - t0); c0 += 16) {
+        uint32_t v[16];
+        tmem_ld16(t_row + c0, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(c0 + i) * kI8Rows] = static_cast<int>(v[i]);
+      }
     }
+    tc_fence_before();
+  }
+  if (splits > 1) {
+    __syncthreads();
+    cluster_sync();
+    if (n_ok && ok) {
+      uint32_t base[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) base[r] = r < splits ? map_shared_rank(smem, r) + (quarter * 32 + lane) * 4 : 0u;
+      for (int c = c_lo; c < c_hi; ++c) {
+        int acc = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < splits) acc += ld_cluster_s32(base[r] + c * (kI8Rows * 4));
+        finish(c, acc);
+      }
+    }
+    __syncthreads();
+    cluster_sync();  // nobody leaves while its partial may still be read
   }
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tbase, cols);
+  }
+}
+
+// ---- many tokens: persistent CTA pairs, 256 tokens x 256 channels per tile ----
+ACCERL_DEVINL void umma_s8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+constexpr int kI8Tile = 256;    // tokens and channels per tile of a CTA pair
+constexpr int kI8Stages = 5;
+constexpr int kI8HalfBytes = 128 * kI8BK;          // a CTA's 128 rows of either operand
+constexpr int kI8StageBytes = 2 * kI8HalfBytes;
+constexpr int kI8EpiChunk = 32 * 128;              // 32 rows x 128 bytes per epilogue warp and buffer
+constexpr int kI8PairSmem = kI8Stages * kI8StageBytes + 4 * 2 * kI8EpiChunk + 2 * 2 * kI8Tile * 4 + 1024;
+static_assert(kI8PairSmem + 1024 <= 232448, "shared memory per CTA");
+
+// tile t -> (token block, channel block), in groups of `group_m` token blocks for L2 reuse of the weight
+ACCERL_DEVINL void int8_tile(const Int8Params& p, int t, int& m_blk, int& n_blk) {
+  const int per_group = p.group_m * p.tiles_n;
+  const int group = t / per_group;
+  const int first = group * p.group_m;
+  const int size = min(p.tiles_m - first, p.group_m);
+  const int r = t % per_group;
+  m_blk = first + r % size;
+  n_blk = r / size;
+}
+
+// The two CTAs of a pair compute one 256 x 256 tile with tcgen05.mma.cta_group::2: each stages its 128
+// tokens and 128 of the channels, the even CTA issues the MMAs, each drains the 128 x 256 accumulator of its
+// tokens. Accumulators are double-buffered in TMEM, so the epilogue of a tile runs under the next one's
+// products. TMA_OUT: the result leaves through swizzled shared memory and TMA stores (16-byte aligned rows);
+// otherwise, and for residuals that are not aligned, through fp32 staging and coalesced element stores.
+template <int OUT, bool TMA_OUT>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                          const __grid_constant__ CUtensorMap tmOut, const Int8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smEpi = smem + kI8Stages * kI8StageBytes;
+  float* sm_scale = reinterpret_cast<float*>(smEpi + 4 * 2 * kI8EpiChunk);  // [buffer][scale, bias][channel]
+  __shared__ uint64_t full[kI8Stages], empty[kI8Stages], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int kbs = (p.K + kI8BK - 1) / kI8BK;
+  const int first = static_cast<int>(blockIdx.x >> 1), stride = static_cast<int>(gridDim.x >> 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kI8Stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 256);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmW);
+  }
+  if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * kI8Tile);
+  tc_fence_before();
+  cluster_sync();  // barriers of both CTAs initialised before any remote signal
+  tc_fence_after();
+  const uint32_t tbase = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, parity = 0;
+      bool ok = true;
+      for (int t = first; t < p.tiles_m * p.tiles_n && ok; t += stride) {
+        int m_blk, n_blk;
+        int8_tile(p, t, m_blk, n_blk);
+        const int m0 = m_blk * kI8Tile + static_cast<int>(rank) * 128, n0 = n_blk * kI8Tile + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, p.status, kStatusTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = map_shared_rank(&full[stage], 0);  // both CTAs' bytes complete the even one's
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kI8StageBytes);
+          uint8_t* dst = smem + stage * kI8StageBytes;
+          tma_load_2d_pair(dst, &tmX, bar, kb * kI8BK, m0);
+          tma_load_2d_pair(dst + kI8HalfBytes, &tmW, bar, kb * kI8BK, n0);
+          issued |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == kI8Stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (ok) {
+        // wait until the MMAs have consumed every stage this CTA filled: no commit may arrive after it left
+        for (int i = 0; i < kI8Stages; ++i) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, p.status, kStatusTimeoutProducer)) break;
+          if (++stage == kI8Stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      } else if (rank == 0) {
+        for (int s = 0; s < kI8Stages; ++s)  // no copy stays in flight into a finished CTA
+          if (issued & (1u << s)) mbar_wait(&full[s], (parity >> s) & 1u, nullptr, 0, 20000000ull);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc_s8_s32(kI8Tile, kI8Tile);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first; t < p.tiles_m * p.tiles_n && ok; t += stride, ++local) {
+        const int acc = local & 1;
+        if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1u, p.status, kStatusTimeoutMma)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!mbar_wait(&full[stage], phase, p.status, kStatusTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t x_addr = smem_u32(smem + stage * kI8StageBytes), w_addr = x_addr + kI8HalfBytes;
+#pragma unroll
+          for (int kk = 0; kk < kI8BK / 32; ++kk)
+            umma_s8_pair(tbase + acc * kI8Tile, make_sw128_desc(x_addr + kk * 32, 16, 1024),
+                         make_sw128_desc(w_addr + kk * 32, 16, 1024), idesc, (kb | kk) != 0);
+          umma_commit_pair(&empty[stage], 0x3);
+          if (++stage == kI8Stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) umma_commit_pair(&tfull[acc], 0x3);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t tempty_even = map_shared_rank(&tempty[0], 0);
+    uint8_t* wbuf = smEpi + quarter * (2 * kI8EpiChunk);
+    int local = 0, chunk = 0;
+    for (int t = first; t < p.tiles_m * p.tiles_n; t += stride, ++local) {
+      int m_blk, n_blk;
+      int8_tile(p, t, m_blk, n_blk);
+      const int acc = local & 1;
+      const int n0 = n_blk * kI8Tile;
+      const int y0 = m_blk * kI8Tile + static_cast<int>(rank) * 128 + quarter * 32;  // first row of this warp
+      const int row = y0 + lane;
+      const bool row_ok = row < p.M;
+      const float sx = row_ok ? __ldg(p.sx + row) : 0.f;
+      // channel scales and bias of the tile, one buffer per accumulator
+      float* scale = sm_scale + acc * 2 * kI8Tile;
+      for (int i = threadIdx.x - 64; i < kI8Tile; i += 128) {
+        const int n = n0 + i;
+        scale[i] = n < p.N ? p.sw[n] : 0.f;
+        scale[kI8Tile + i] = (n < p.N && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
+      }
+      // the four warps go on, or give up, together
+      if (!named_bar_and(1, 128, mbar_wait(&tfull[acc], (local >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
+      tc_fence_after();
+      const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kI8Tile;
+      constexpr int kCols = (TMA_OUT && OUT != kOutF32) ? 64 : 32;  // columns per 4 KB buffer
+#pragma unroll 1
+      for (int c0 = 0; c0 < kI8Tile && n0 + c0 < p.N; c0 += kCols) {
+        uint8_t* buf = wbuf + (chunk & 1) * kI8EpiChunk;
+        ++chunk;
+        if constexpr (TMA_OUT) {
+          if (lane == 0) bulk_wait_read<1>();  // the store issued from this buffer two chunks ago
+        }
+        __syncwarp();
+        uint32_t v[kCols];
+#pragma unroll
+        for (int h = 0; h < kCols; h += 32) tmem_ld32(t_row + c0 + h, *reinterpret_cast<uint32_t(*)[32]>(v + h));
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // 16-byte pieces of the staged row
+          constexpr int kPer = kCols / 8;
+          float f[kPer];
+#pragma unroll
+          for (int i = 0; i < kPer; i += 4) {
+            const int c = c0 + j * kPer + i;
+            const float4 s4 = *reinterpret_cast<const float4*>(scale + c);
+            const float4 b4 = *reinterpret_cast<const float4*>(scale + kI8Tile + c);
+            f[i] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i])), sx * s4.x, b4.x);
+            f[i + 1] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i + 1])), sx * s4.y, b4.y);
+            f[i + 2] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i + 2])), sx * s4.z, b4.z);
+            f[i + 3] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i + 3])), sx * s4.w, b4.w);
+          }
+          if constexpr (TMA_OUT) {
+            if (p.residual && row_ok) {
+              // aligned rows: whole pieces lie inside the row's allocation when their first column does
+              const int col = n0 + c0 + j * kPer;
+              const long long at = row * p.ldr + col;
+              if (col + kPer <= p.N) {
+                if (p.in_type == kOutF32) {
+#pragma unroll
+                  for (int i = 0; i < kPer; i += 4) {
+                    const float4 r = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + at + i);
+                    f[i] += r.x;
+                    f[i + 1] += r.y;
+                    f[i + 2] += r.z;
+                    f[i + 3] += r.w;
+                  }
+                } else {
+#pragma unroll
+                  for (int i = 0; i < kPer; i += 4) {
+                    const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p.residual) + at + i);
+                    const float2 a = p.in_type == kOutBf16 ? Half16<__nv_bfloat16>::unpack(r.x) : Half16<__half>::unpack(r.x);
+                    const float2 b = p.in_type == kOutBf16 ? Half16<__nv_bfloat16>::unpack(r.y) : Half16<__half>::unpack(r.y);
+                    f[i] += a.x;
+                    f[i + 1] += a.y;
+                    f[i + 2] += b.x;
+                    f[i + 3] += b.y;
+                  }
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                  if (col + i < p.N) f[i] += load_as_float(p.residual, at + i, p.in_type);
+              }
+            }
+          }
+          uint4 o;
+          if constexpr (TMA_OUT && OUT == kOutBf16)
+            o = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+          else if constexpr (TMA_OUT && OUT == kOutF16)
+            o = make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
+          else
+            o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+          *reinterpret_cast<uint4*>(buf + swz128(lane, j)) = o;
+        }
+        if constexpr (TMA_OUT) {
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmOut, buf, n0 + c0, y0);
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          const int n = n0 + c0 + lane;
+          if (n < p.N) {
+            for (int r = 0; r < 32 && y0 + r < p.M; ++r) {
+              float y = *reinterpret_cast<const float*>(buf + swz128(r, lane >> 2) + (lane & 3) * 4);
+              const long long at = y0 + r;
+              if (p.residual) y += load_as_float(p.residual, at * p.ldr + n, p.in_type);
+              store_from_float(p.out, at * p.ldo + n, OUT, y);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      mbar_arrive_cluster(tempty_even + acc * 8);
+    }
+    if (TMA_OUT && lane == 0) bulk_wait<0>();
+  }
+  __syncthreads();
+  tc_fence_before();
+  cluster_sync();  // neither CTA leaves while the other may still signal into its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tbase, 2 * kI8Tile);
   }
 }
 
@@ -404,6 +726,60 @@ bool make_int8_map(CUtensorMap* out, const void* ptr, uint64_t pitch, uint64_t r
   return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Map of the output for tiles of 128 bytes x 32 rows. False when TMA cannot store it (alignment).
+bool make_out_map(CUtensorMap* out, const Int8Params& p) {
+  const uint64_t es = p.out_type == kOutF32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(p.out) & 15) || (p.ldo * es) % 16 || p.ldo < p.N) return false;
+  auto fn = int8_encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.N), static_cast<cuuint64_t>(p.M)};
+  cuuint64_t strides[1] = {p.ldo * es};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType dt = p.out_type == kOutF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : p.out_type == kOutF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(out, dt, 2, p.out, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaLaunchConfig_t cluster_config(dim3 grid, int smem, cudaStream_t s, cudaLaunchAttribute* attr, unsigned x, unsigned z) {
+  cudaLaunchConfig_t cfg = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = x;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = z;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kI8Threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+template <int OUT, bool TMA_OUT>
+int launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Int8Params& p, cudaStream_t s) {
+  auto kern = gemm_int8_pair_kernel<OUT, TMA_OUT>;
+  static std::atomic<int> cache[kMaxHostDevices];  // pairs that can be resident at once, per device
+  const int dev = host_current_device();
+  if (dev < 0 || dev >= kMaxHostDevices) return -14;
+  cudaLaunchAttribute attr[1];
+  int pairs = cache[dev].load(std::memory_order_acquire);
+  if (pairs == 0) {
+    cudaError_t e = smem_attr_once<gemm_int8_pair_kernel<OUT, TMA_OUT>>(kI8PairSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    cudaLaunchConfig_t cfg = cluster_config(dim3(2 * (device_sm_count() / 2)), kI8PairSmem, s, attr, 2, 1);
+    e = cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (pairs < 1) return -13;
+    cache[dev].store(pairs, std::memory_order_release);
+  }
+  const int grid = 2 * std::min(pairs, p.tiles_m * p.tiles_n);
+  cudaLaunchConfig_t cfg = cluster_config(dim3(grid), kI8PairSmem, s, attr, 2, 1);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, mx, mw, mo, p));
 }
 
 template <typename T, int PRE>
@@ -480,20 +856,44 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   p.out_type = out_type;
   p.in_type = in_type;
   p.status = status;
+  p.tiles_m = (M + kI8Tile - 1) / kI8Tile;
+  p.tiles_n = (N + kI8Tile - 1) / kI8Tile;
+  p.group_m = 8;
+  if (M > 256) {
+    CUtensorMap mx, mw, mo;
+    if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), 128)) return -7;
+    if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), 128)) return -8;
+    const int rs = in_type == kOutF32 ? 4 : 2;
+    const bool res_ok = !residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * rs) % 16 == 0);
+    if (static_cast<long long>(p.tiles_m) * p.tiles_n > 0x3fffffff) return -4;
+    if (res_ok && make_out_map(&mo, p)) {
+      if (out_type == kOutBf16) return launch_pair<kOutBf16, true>(mx, mw, mo, p, stream);
+      if (out_type == kOutF16) return launch_pair<kOutF16, true>(mx, mw, mo, p, stream);
+      return launch_pair<kOutF32, true>(mx, mw, mo, p, stream);
+    }
+    mo = mx;
+    if (out_type == kOutBf16) return launch_pair<kOutBf16, false>(mx, mw, mo, p, stream);
+    if (out_type == kOutF16) return launch_pair<kOutF16, false>(mx, mw, mo, p, stream);
+    return launch_pair<kOutF32, false>(mx, mw, mo, p, stream);
+  }
   p.bt = 16;
-  while (p.bt < M && p.bt < kI8MaxTokens) p.bt *= 2;
+  while (p.bt < M) p.bt *= 2;
   const int kbs = (K + kI8BK - 1) / kI8BK;
+  const int tiles = (N + kI8Rows - 1) / kI8Rows;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= device_sm_count() && splits * 2 <= kbs) splits *= 2;
   const int stage_bytes = (kI8Rows + p.bt) * kI8BK;
-  p.stages = std::max(2, std::min({16, kbs, 200 * 1024 / stage_bytes}));
-  const int smem_bytes = p.stages * stage_bytes + 1024;
+  const int budget = tiles * splits > device_sm_count() ? 100 * 1024 : 200 * 1024;
+  p.stages = std::max(2, std::min({16, (kbs + splits - 1) / splits, budget / stage_bytes}));
+  int smem_bytes = p.stages * stage_bytes;
+  if (splits > 1) smem_bytes = std::max(smem_bytes, p.bt * kI8Rows * 4);  // the partial
+  smem_bytes += 1024;
   CUtensorMap mw, mx;
   if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), kI8Rows)) return -7;
   if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), static_cast<uint32_t>(p.bt))) return -8;
-  cudaError_t e = smem_attr_once<gemm_int8_kernel>(16 * 1024 + 200 * 1024);
+  cudaError_t e = smem_attr_once<gemm_int8_stream_kernel>(201 * 1024);
   if (e != cudaSuccess) return static_cast<int>(e);
-  const long long tiles_t = (static_cast<long long>(M) + p.bt - 1) / p.bt;
-  if (tiles_t > 65535) return -4;
-  const dim3 grid((N + kI8Rows - 1) / kI8Rows, static_cast<unsigned>(tiles_t));
-  gemm_int8_kernel<<<grid, kI8Threads, smem_bytes, stream>>>(mw, mx, p);
-  return static_cast<int>(cudaGetLastError());
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = cluster_config(dim3(tiles, 1, splits), smem_bytes, stream, attr, 1, splits);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_stream_kernel, mw, mx, p));
 }
