@@ -19,7 +19,7 @@ from ._ext import available, check_status, debug_checks_enabled, debug_status, n
 
 # Kernels launched by one call of each binding (the benchmark reports launches per timed step).
 KERNELS_PER_CALL = {
-    "rmsnorm_bwd": 3, "bias_grad": 2, "attn_bwd": 4, "paged_decode": 2, "sample_logits": 2,
+    "rmsnorm_bwd": 3, "bias_grad": 2, "attn_bwd": 4, "paged_decode": 2, "sample_logits": 2, "linear_int8": 2,
 }
 LAUNCHES = [0]
 
@@ -37,11 +37,12 @@ class _Checked:
         last_error = self._ext.last_error
 
         def call(*args):
-            fn(*args)
+            res = fn(*args)
             LAUNCHES[0] += per_call
             rc, msg = last_error()
             if rc != 0:
                 raise RuntimeError(f"native op {name} failed (code {rc}): {msg}")
+            return res
 
         self.__dict__[name] = call  # later lookups find the wrapper without __getattr__
         return call
@@ -347,24 +348,38 @@ class Int8Rows:
         return self.q[:, : self.k].float() * self.scale.unsqueeze(1)
 
 
-def _int8_rows(rows: int, k: int, device: torch.device, out: Optional[Int8Rows]) -> Int8Rows:
+def _quantize(x: torch.Tensor, pre: int, w, eps: float, out: Optional[Int8Rows]) -> Int8Rows:
+    """Rows to 8 bits on x's device; the CUDA entry makes the same checks as the ones below."""
+    if x.is_cuda:
+        k = x.shape[-1] // 2 if pre == 2 else x.shape[-1]
+        if out is None:
+            q, scale = native().quantize_rows(x, pre, w, eps, None, None)
+            return Int8Rows(q, scale, k)
+        if out.k != k:
+            raise ValueError(f"out does not hold rows of {k}")
+        native().quantize_rows(x, pre, w, eps, out.q, out.scale)
+        return out
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x must be [rows, features], got {tuple(x.shape)}")
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        raise ValueError("the last dimension of x must be contiguous")
+    if pre == 2 and x.shape[1] % 2:
+        raise ValueError("gate | up must be [rows, 2K]")
+    if pre == 1 and (w.numel() != x.shape[1] or w.device != x.device):
+        raise ValueError(f"the norm weight must be [{x.shape[1]}] on x's device")
+    rows, k = x.shape[0], x.shape[1] // 2 if pre == 2 else x.shape[1]
     kp = (k + 15) // 16 * 16
     if out is None:
-        return Int8Rows(torch.empty(rows, kp, dtype=torch.int8, device=device),
-                        torch.empty(rows, dtype=torch.float32, device=device), k)
-    if (out.k != k or tuple(out.q.shape) != (rows, kp) or out.scale.numel() != rows or out.q.device != device
-            or out.scale.device != device or out.q.dtype != torch.int8 or out.scale.dtype != torch.float32):
-        raise ValueError(f"out does not hold {rows} x {k} int8 rows on {device}")
+        out = Int8Rows(torch.empty(rows, kp, dtype=torch.int8), torch.empty(rows), k)
+    elif (out.k != k or tuple(out.q.shape) != (rows, kp) or out.scale.numel() != rows or out.q.device != x.device
+          or out.q.dtype != torch.int8 or out.scale.dtype != torch.float32):
+        raise ValueError(f"out does not hold {rows} x {k} int8 rows on {x.device}")
+    if pre == 1:
+        x = reference.rmsnorm(x, w, eps)[0]
+    elif pre == 2:
+        x = reference.swiglu(x)
+    reference.quantize_rows(x, out.q, out.scale)
     return out
-
-
-def _check_rows(name: str, x: torch.Tensor, dtypes) -> None:
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"{name} must be [rows, features], got {tuple(x.shape)}")
-    if x.is_cuda and x.dtype not in dtypes:
-        raise ValueError(f"{name} must be {' or '.join(str(d).split('.')[-1] for d in dtypes)}, got {x.dtype}")
-    if x.shape[1] > 1 and x.stride(1) != 1:
-        raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
 def quantize_rows(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
@@ -373,46 +388,20 @@ def quantize_rows(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     0; a row with an infinity or NaN has scale NaN and zeros, so every product with it is NaN.
 
     Rows may be strided; sizes and strides that are multiples of 8 take 16-byte accesses."""
-    _check_rows("x", x, (torch.bfloat16, torch.float16))
-    out = _int8_rows(x.shape[0], x.shape[1], x.device, out)
-    if x.is_cuda:
-        native().quantize_rows(x, 0, None, 0.0, out.q, out.scale)
-    else:
-        reference.quantize_rows(x, out.q, out.scale)
-    return out
+    return _quantize(x, 0, None, 0.0, out)
 
 
 def rmsnorm_quantize(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[Int8Rows] = None) -> Int8Rows:
     """``quantize_rows(rmsnorm(x, w, eps)[0])`` in one pass over ``x`` (bf16 [rows, K]; on the GPU K is a
-    multiple of 8 up to 32768). The normalised rows are rounded to bf16 as ``rmsnorm`` rounds them."""
-    _check_rows("x", x, (torch.bfloat16,))
-    if w.numel() != x.shape[1] or w.device != x.device or (x.is_cuda and w.dtype != x.dtype):
-        raise ValueError("the norm weight must be [K], of x's type and on x's device")
-    out = _int8_rows(x.shape[0], x.shape[1], x.device, out)
-    if x.is_cuda:
-        if x.shape[1] % 8 or x.shape[1] > 32768 or x.stride(0) % 8 or x.data_ptr() % 16 or w.data_ptr() % 16:
-            raise ValueError("rmsnorm_quantize needs rows of a multiple of 8 (at most 32768) elements, aligned to 16 bytes")
-        native().quantize_rows(x, 1, w.contiguous(), eps, out.q, out.scale)
-    else:
-        reference.quantize_rows(reference.rmsnorm(x, w, eps)[0], out.q, out.scale)
-    return out
+    multiple of 8 up to 32768 and rows and weight are aligned to 16 bytes). The normalised rows are rounded
+    to bf16 as ``rmsnorm`` rounds them."""
+    return _quantize(x, 1, w, eps, out)
 
 
 def swiglu_quantize(gu: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     """``quantize_rows(swiglu(gu))`` in one pass over ``gu`` = gate | up (bf16 [rows, 2K]; on the GPU K is a
-    multiple of 8 up to 32768). Same bits as the two calls."""
-    _check_rows("gu", gu, (torch.bfloat16,))
-    if gu.shape[1] % 2:
-        raise ValueError("gu must be [rows, 2K]")
-    k = gu.shape[1] // 2
-    out = _int8_rows(gu.shape[0], k, gu.device, out)
-    if gu.is_cuda:
-        if k % 8 or k > 32768 or gu.stride(0) % 8 or gu.data_ptr() % 16:
-            raise ValueError("swiglu_quantize needs K a multiple of 8 (at most 32768) and rows aligned to 16 bytes")
-        native().quantize_rows(gu, 2, None, 0.0, out.q, out.scale)
-    else:
-        reference.quantize_rows(reference.swiglu(gu), out.q, out.scale)
-    return out
+    multiple of 8 up to 32768 and rows are aligned to 16 bytes)."""
+    return _quantize(gu, 2, None, 0.0, out)
 
 
 def linear_int8(x: Union[torch.Tensor, Int8Rows], w: Int8Rows, bias: Optional[torch.Tensor] = None,
@@ -428,13 +417,20 @@ def linear_int8(x: Union[torch.Tensor, Int8Rows], w: Int8Rows, bias: Optional[to
     ``out`` itself. ``in`` is at most ``INT8_MAX_K``."""
     if not isinstance(w, Int8Rows):
         raise ValueError("w must be Int8Rows: quantize_rows(weight)")
+    if w.q.is_cuda:  # the checks below are made by the CUDA entries
+        status = status_tensor(w.q.device)
+        if not isinstance(x, Int8Rows):
+            return native().linear_int8(x, w.q, w.scale, w.k, bias, residual, out, out_dtype, status)
+        if x.k != w.k:
+            raise ValueError(f"inner dimensions differ ({x.k} vs {w.k})")
+        return native().gemm_int8(x.q, x.scale, w.q, w.scale, w.k, bias, residual, out, out_dtype or torch.bfloat16,
+                                  status, False)
     if not isinstance(x, Int8Rows):
         out_dtype = out_dtype or x.dtype
-        if x.dim() == 2 and x.shape[1] != w.k:
-            raise ValueError(f"inner dimensions differ ({x.shape[1]} vs {w.k})")
+        if x.dim() != 2 or x.shape[1] != w.k:
+            raise ValueError(f"inner dimensions differ ({tuple(x.shape)} vs {w.k})")
         x = quantize_rows(x)
     M, N, K = x.q.shape[0], w.q.shape[0], w.k
-    dev = w.q.device
     if x.k != K:
         raise ValueError(f"inner dimensions differ ({x.k} vs {K})")
     if K > INT8_MAX_K:
@@ -444,24 +440,21 @@ def linear_int8(x: Union[torch.Tensor, Int8Rows], w: Int8Rows, bias: Optional[to
         out_dtype = out_dtype or torch.bfloat16
         if out_dtype not in floats:
             raise ValueError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
-        out = torch.empty(M, N, dtype=out_dtype, device=dev)
-    elif tuple(out.shape) != (M, N) or out.dtype not in floats or (N > 1 and out.stride(1) != 1):
+        out = torch.empty(M, N, dtype=out_dtype)
+    elif (tuple(out.shape) != (M, N) or out.dtype not in floats or (N > 1 and out.stride(1) != 1)
+          or (M > 1 and out.stride(0) < N)):
         raise ValueError(f"out must be bf16, fp16 or fp32 [{M}, {N}] with a contiguous last dimension")
-    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in floats or not bias.is_contiguous()):
-        raise ValueError(f"bias must be contiguous bf16, fp16 or fp32 [{N}]")
     if residual is not None and (tuple(residual.shape) != (M, N) or residual.dtype not in floats
                                  or (N > 1 and residual.stride(1) != 1)):
         raise ValueError(f"residual must be bf16, fp16 or fp32 [{M}, {N}] with a contiguous last dimension")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in floats or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous bf16, fp16 or fp32 [{N}]")
     if bias is not None and residual is not None and bias.dtype != residual.dtype:
         raise ValueError("bias and residual must be of one type")
     for t in (x.q, x.scale, w.scale, out, bias, residual):
-        if t is not None and t.device != dev:
-            raise ValueError(f"every tensor must be on the weight's device {dev}, got one on {t.device}")
-    if dev.type == "cuda":
-        native().gemm_int8(x.q, x.scale, w.q, w.scale, K, bias, residual, out, status_tensor(dev))
-    else:
-        out.copy_(reference.linear_int8(x.q, x.scale, w.q, w.scale, bias, residual))
-    return out
+        if t is not None and t.device != w.q.device:
+            raise ValueError(f"every tensor must be on the weight's device {w.q.device}, got one on {t.device}")
+    return out.copy_(reference.linear_int8(x.q, x.scale, w.q, w.scale, bias, residual))
 
 
 # ------------------------------------------------------------------------------------------------

@@ -129,7 +129,7 @@ int accerl_quantize_rows(const void* x, long long ldx, int half, int pre, const 
                          float* scale, long long rows, int K, cudaStream_t s);
 int accerl_gemm_int8(const void* qx, const float* sx, const void* qw, const float* sw, int M, int N, int K,
                      const void* bias, const void* residual, long long ldr, int in_type, void* out, long long ldo,
-                     int out_type, int* status, cudaStream_t stream);
+                     int out_type, int w_early, int* status, cudaStream_t stream);
 }
 
 namespace {
@@ -810,73 +810,124 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
 }
 
 // x [rows, K] (pre 0: as it is, 1: RMSNorm with weight w, 2: SwiGLU of gate | up [rows, 2K]) -> int8 rows
-// q [rows, K rounded up to 16] and scale [rows].
-void quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w, double eps, at::Tensor& q,
-                   at::Tensor& scale) {
+// q [rows, K rounded up to 16] and scale [rows], allocated when not given.
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w,
+                                                 double eps, const c10::optional<at::Tensor>& q_out,
+                                                 const c10::optional<at::Tensor>& scale_out) {
   const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
-  CHECK_CUDA(x);
-  CHECK_CUDA(q);
-  CHECK_CUDA(scale);
-  CHECK_F32(scale);
-  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "quantize_rows: bf16 or fp16 rows");
-  const int64_t K = pre == 2 ? x.size(1) / 2 : x.size(1);
-  TORCH_CHECK(q.scalar_type() == at::kChar && q.is_contiguous() && q.size(0) == x.size(0) &&
-                  q.size(1) == (K + 15) / 16 * 16,
-              "quantize_rows: q must be int8 [rows, K rounded up to 16]");
-  TORCH_CHECK(scale.is_contiguous() && scale.numel() == x.size(0), "quantize_rows: scale [rows]");
-  if (pre == 1) {
-    TORCH_CHECK(w.has_value() && w->is_cuda() && w->numel() == K && w->is_contiguous(), "quantize_rows: norm weight [K]");
-    CHECK_BF16(*w);
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be [rows, features], got ", x.sizes());
+  const bool half = x.scalar_type() == at::kHalf;
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || (half && pre == 0), "x must be bfloat16",
+                    pre == 0 ? " or float16" : "", ", got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.stride(1) == 1 || x.size(1) == 1, "the last dimension of x must be contiguous");
+  TORCH_CHECK_VALUE(pre != 2 || x.size(1) % 2 == 0, "gate | up must be [rows, 2K]");
+  const int64_t rows = x.size(0), K = pre == 2 ? x.size(1) / 2 : x.size(1), Kp = (K + 15) / 16 * 16;
+  TORCH_CHECK_VALUE(rows <= 0x7fffffff && K < 0x7fffff00, "too many rows or features: ", x.sizes());
+  if (pre != 0) {
+    const bool aligned = K % 8 == 0 && K <= 32768 && (rows <= 1 || x.stride(0) % 8 == 0) &&
+                         reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    TORCH_CHECK_VALUE(aligned, "K must be a multiple of 8, at most 32768, and the rows aligned to 16 bytes");
   }
-  check(accerl_quantize_rows(x.data_ptr(), ld_of(x), x.scalar_type() == at::kHalf, static_cast<int>(pre), opt_ptr(w),
-                             static_cast<float>(eps), q.data_ptr(), scale.data_ptr<float>(), x.size(0),
-                             static_cast<int>(K), cur_stream()),
+  if (pre == 1) {
+    TORCH_CHECK_VALUE(w.has_value() && w->numel() == K && w->is_contiguous() && w->device() == x.device() &&
+                          w->scalar_type() == at::kBFloat16 && reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0,
+                      "the norm weight must be contiguous bfloat16 [", K, "] on x's device, aligned to 16 bytes");
+  }
+  at::Tensor q, scale;
+  if (q_out.has_value()) {
+    q = *q_out;
+    scale = *scale_out;
+    TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.is_contiguous() && q.dim() == 2 && q.size(0) == rows &&
+                          q.size(1) == Kp && scale.scalar_type() == at::kFloat && scale.is_contiguous() &&
+                          scale.numel() == rows && q.device() == x.device() && scale.device() == x.device(),
+                      "out does not hold ", rows, " x ", K, " int8 rows on ", x.device());
+  } else {
+    q = at::empty({rows, Kp}, x.options().dtype(at::kChar));
+    scale = at::empty({rows}, x.options().dtype(at::kFloat));
+  }
+  check(accerl_quantize_rows(x.data_ptr(), rows <= 1 ? 0 : x.stride(0), half, static_cast<int>(pre), opt_ptr(w),
+                             static_cast<float>(eps), q.data_ptr(), scale.data_ptr<float>(), rows, static_cast<int>(K),
+                             cur_stream()),
         "quantize_rows");
+  return {q, scale};
 }
 
-int float_type_id(const at::Tensor& t) {
-  if (t.scalar_type() == at::kBFloat16) return 0;
-  if (t.scalar_type() == at::kHalf) return 1;
-  TORCH_CHECK(t.scalar_type() == at::kFloat, "expected bf16, fp16 or f32");
-  return 2;
+// 0 bf16, 1 fp16, 2 fp32, -1 anything else
+int float_type_id(at::ScalarType t) {
+  return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1;
 }
 
-// out [M, N] = sx sw (qx qw^T) (+ bias) (+ residual); bias and residual share one type
-void gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
-               const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, at::Tensor& out,
-               const c10::optional<at::Tensor>& status) {
-  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(qx));
-  CHECK_CUDA(qx);
-  CHECK_CUDA(qw);
-  CHECK_CUDA(out);
-  CHECK_F32(sx);
-  CHECK_F32(sw);
+// out [M, N] = sx sw (qx qw^T) (+ bias) (+ residual), out allocated when not given
+at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
+                     const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                     const c10::optional<at::Tensor>& out_opt, const c10::optional<at::ScalarType>& out_dtype,
+                     const at::Tensor& status, bool w_early) {
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(qw));
   const int64_t M = qx.size(0), N = qw.size(0), Kp = (K + 15) / 16 * 16;
-  TORCH_CHECK(qx.scalar_type() == at::kChar && qw.scalar_type() == at::kChar, "gemm_int8: int8 operands");
-  TORCH_CHECK(qx.is_contiguous() && qw.is_contiguous() && qx.size(1) == Kp && qw.size(1) == Kp,
-              "gemm_int8: operands must be contiguous [rows, K rounded up to 16]");
-  TORCH_CHECK(sx.is_cuda() && sw.is_cuda() && sx.is_contiguous() && sw.is_contiguous() && sx.numel() == M &&
-                  sw.numel() == N,
-              "gemm_int8: one scale per row");
-  TORCH_CHECK(out.size(0) == M && out.size(1) == N, "gemm_int8: output shape mismatch");
-  int in_type = float_type_id(out);
+  const auto dev = qw.device();
+  auto on_device = [&](const at::Tensor& t) {
+    TORCH_CHECK_VALUE(t.device() == dev, "every tensor must be on the weight's device ", dev, ", got one on ", t.device());
+  };
+  on_device(qx), on_device(sx), on_device(sw);
+  TORCH_CHECK_VALUE(K > 0 && K <= 133144, "in must be at most 133144, got ", K);
+  for (const at::Tensor* q : {&qx, &qw})
+    TORCH_CHECK_VALUE(q->scalar_type() == at::kChar && q->dim() == 2 && q->is_contiguous() && q->size(1) == Kp &&
+                          reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 == 0,
+                      "int8 rows must be contiguous [rows, in rounded up to 16], aligned to 16 bytes");
+  TORCH_CHECK_VALUE(sx.scalar_type() == at::kFloat && sw.scalar_type() == at::kFloat && sx.is_contiguous() &&
+                        sw.is_contiguous() && sx.numel() == M && sw.numel() == N,
+                    "int8 rows must have one contiguous float32 scale each");
+  TORCH_CHECK_VALUE(M <= 0x3fffffff && N <= 0x3fffffff, "too many rows");
+  at::Tensor out;
+  if (out_opt.has_value()) {
+    out = *out_opt;
+    TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == M && out.size(1) == N && float_type_id(out.scalar_type()) >= 0 &&
+                          (N <= 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N),
+                      "out must be bf16, fp16 or fp32 [", M, ", ", N, "] with a contiguous last dimension");
+    on_device(out);
+  } else {
+    TORCH_CHECK_VALUE(out_dtype.has_value() && float_type_id(*out_dtype) >= 0, "out_dtype must be bf16, fp16 or fp32");
+    out = at::empty({M, N}, qw.options().dtype(*out_dtype));
+  }
+  int in_type = float_type_id(out.scalar_type());
   long long ldr = 0;
   if (residual.has_value()) {
-    TORCH_CHECK(residual->is_cuda() && residual->size(0) == M && residual->size(1) == N,
-                "gemm_int8: residual shape mismatch");
-    in_type = float_type_id(*residual);
-    ldr = ld_of(*residual);
+    TORCH_CHECK_VALUE(residual->dim() == 2 && residual->size(0) == M && residual->size(1) == N &&
+                          float_type_id(residual->scalar_type()) >= 0 && (N <= 1 || residual->stride(1) == 1),
+                      "residual must be bf16, fp16 or fp32 [", M, ", ", N, "] with a contiguous last dimension");
+    on_device(*residual);
+    in_type = float_type_id(residual->scalar_type());
+    ldr = residual->stride(0);
   }
   if (bias.has_value()) {
-    TORCH_CHECK(bias->is_cuda() && bias->numel() == N && bias->is_contiguous(), "gemm_int8: bias must be contiguous [N]");
-    TORCH_CHECK(!residual.has_value() || float_type_id(*bias) == in_type, "gemm_int8: bias and residual types differ");
-    in_type = float_type_id(*bias);
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->numel() == N && bias->is_contiguous() &&
+                          float_type_id(bias->scalar_type()) >= 0,
+                      "bias must be contiguous bf16, fp16 or fp32 [", N, "]");
+    on_device(*bias);
+    TORCH_CHECK_VALUE(!residual.has_value() || bias->scalar_type() == residual->scalar_type(),
+                      "bias and residual must be of one type");
+    in_type = float_type_id(bias->scalar_type());
   }
   check(accerl_gemm_int8(qx.data_ptr(), sx.data_ptr<float>(), qw.data_ptr(), sw.data_ptr<float>(),
                          static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), opt_ptr(bias),
-                         opt_ptr(residual), ldr, in_type, out.data_ptr(), ld_of(out), float_type_id(out),
-                         status_ptr(status), cur_stream()),
+                         opt_ptr(residual), ldr, in_type, out.data_ptr(), M <= 1 ? N : out.stride(0),
+                         float_type_id(out.scalar_type()), w_early, status.data_ptr<int>(), cur_stream()),
         "gemm_int8");
+  return out;
+}
+
+// The same from bf16 / fp16 activations: quantised first, the product launched to start behind that kernel.
+at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
+                       const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                       const c10::optional<at::Tensor>& out, const c10::optional<at::ScalarType>& out_dtype,
+                       const at::Tensor& status) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "inner dimensions differ (", x.sizes(), " vs ", K, ")");
+  TORCH_CHECK_VALUE(x.device() == qw.device(), "every tensor must be on the weight's device ", qw.device(),
+                    ", got one on ", x.device());
+  auto [qx, sx] = quantize_rows(x, 0, c10::nullopt, 0.0, c10::nullopt, c10::nullopt);
+  if (g_last_rc != 0) return qx;  // reported by the caller
+  return gemm_int8(qx, sx, qw, sw, K, bias, residual, out, out_dtype.has_value() ? out_dtype : x.scalar_type(), status,
+                   true);
 }
 
 }  // namespace
@@ -1000,6 +1051,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample_counts", &sample_counts, "one token per row from given uniform numbers");
   m.def("quantize_rows", &quantize_rows, "rows to int8 with a scale each, optionally behind RMSNorm or SwiGLU");
   m.def("gemm_int8", &gemm_int8, "tcgen05 int8 GEMM with token and channel scales");
+  m.def("linear_int8", &linear_int8, "rows to int8 and their product");
   m.def("enable_peer_access", &enable_peer_access);
   m.def("rs_sumsq", &rs_sumsq);
   m.def("adamw_push", &adamw_push);

@@ -19,6 +19,11 @@ namespace accerl {
 // ------------------------------------------------------------------------------------------------
 // rows to 8 bits
 // ------------------------------------------------------------------------------------------------
+// Programmatic dependent launch: a product launched behind its quantising kernel starts while that one still
+// runs, sets itself up and waits here for the whole grid before it and its memory.
+ACCERL_DEVINL void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+ACCERL_DEVINL void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 enum QuantPre : int { kPreNone = 0, kPreRmsNorm = 1, kPreSwiglu = 2 };
 
 template <typename T>
@@ -61,9 +66,10 @@ ACCERL_DEVINL RowQuant row_quant(uint32_t amax) {
 
 // round_half_even(127 x / a), decided exactly without a division per element. x and a have at most 11
 // significant bits, so the quotient is either a whole number and a half or at least a relative 2^-19 away
-// from every such border. p is within 2^-23 of it; the remainder 127 x - p a is exact, and the corrected
-// quotient is the exact one where that is representable, which every border is. The last addition rounds to
-// the nearest whole number, ties to even; the low byte of its pattern is the two's complement.
+// from every such border. p is within 2^-22 of it; the remainder 127 x - p a is exact, and the quotient
+// corrected by it (Markstein, 1990) is the exact one where that is representable, which every border is. The
+// last addition rounds to the nearest whole number, ties to even; the low byte of its pattern is the two's
+// complement.
 ACCERL_DEVINL uint32_t quant_bits(float x, const RowQuant& s) {
   const float n = __fmul_rn(x, s.m127);
   const float p = __fmul_rn(n, s.inv);
@@ -74,19 +80,30 @@ ACCERL_DEVINL uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Reduction over the `tpr` threads of a row (a power of two, 32..blockDim); `red` has one slot per warp.
+// silu(g) u with the activation rounded to bf16, as swiglu_h gives it, without its division, which kept this
+// kernel at the instruction limit: the quotient g / (1 + e^-g) from an approximate reciprocal, corrected by its
+// exact remainder (Markstein, 1990). Gates beyond 80, where remainder or reciprocal could leave the normal
+// range, take swiglu_h itself.
+ACCERL_DEVINL float swiglu_row(float g, float u) {
+  if (!(fabsf(g) < 80.f)) return swiglu_h(g, u);
+  const float d = 1.f + __expf(-g);
+  const float r = __fdividef(1.f, d);
+  const float q = __fmul_rn(g, r);
+  return bf16_round(__fmaf_rn(__fmaf_rn(-q, d, g), r, q)) * u;
+}
+
+// Reduction over the `tpr` threads of a row (a power of two, 32..blockDim); `red`, one slot per warp, is used
+// by one reduction of the kernel only.
 template <typename V, typename F>
 ACCERL_DEVINL V row_reduce(V v, int tpr, V* red, F f) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (tpr > 32) {
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     const int w0 = (threadIdx.x / tpr) * (tpr >> 5);
     v = red[w0];
     for (int w = 1; w < (tpr >> 5); ++w) v = f(v, red[w0 + w]);
-    __syncthreads();
   }
   return v;
 }
@@ -98,32 +115,36 @@ ACCERL_DEVINL uint32_t amax_pair(uint32_t m) { return max(m & 0xffffu, m >> 16);
 // (x [rows, K], weight w) or SwiGLU (x = gate | up, [rows, 2K]), with the roundings of the framework's
 // own kernels (both give rows in T).
 template <typename T, int PRE, int NC>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict__ x, long long ldx,
-                                                             const T* __restrict__ w, float eps,
-                                                             int8_t* __restrict__ q, float* __restrict__ scale,
-                                                             long long rows, int K, int Kp, int tpr) {
-  __shared__ uint32_t red_u[32];
-  __shared__ float red_f[32];
+__global__ void __launch_bounds__(512) quantize_rows_kernel(const T* __restrict__ x, long long ldx,
+                                                            const T* __restrict__ w, float eps,
+                                                            int8_t* __restrict__ q, float* __restrict__ scale,
+                                                            long long rows, int K, int Kp, int tpr) {
+  pdl_launch_dependents();  // the product may set itself up; it waits for this grid's end before it reads
+  __shared__ uint32_t red_u[16];
+  __shared__ float red_f[16];
   const int in_row = threadIdx.x % tpr;
   const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
   const bool live = row < rows;
   const T* xr = x + (live ? row : 0) * ldx;
-  uint4 v[NC];
+  // every load of the row is issued up front; chunks behind its end read its first one and are zeroed
+  uint4 v[NC], up[PRE == kPreSwiglu ? NC : 1];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const int c = (j * tpr + in_row) * 8;
-    v[j] = make_uint4(0, 0, 0, 0);
-    if (live && c < K) {
-      v[j] = *reinterpret_cast<const uint4*>(xr + c);
-      if constexpr (PRE == kPreSwiglu) {
-        const uint4 u = *reinterpret_cast<const uint4*>(xr + K + c);
-        uint32_t* g = reinterpret_cast<uint32_t*>(&v[j]);
-        const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+    v[j] = *reinterpret_cast<const uint4*>(xr + (c < K ? c : 0));
+    if constexpr (PRE == kPreSwiglu) up[j] = *reinterpret_cast<const uint4*>(xr + K + (c < K ? c : 0));
+  }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 fg = unpack_bf16x2(g[i]), fu = unpack_bf16x2(uw[i]);
-          g[i] = pack_bf16x2(swiglu_h(fg.x, fu.x), swiglu_h(fg.y, fu.y));
-        }
+  for (int j = 0; j < NC; ++j) {
+    if ((j * tpr + in_row) * 8 >= K) {
+      v[j] = make_uint4(0, 0, 0, 0);
+    } else if constexpr (PRE == kPreSwiglu) {
+      uint32_t* g = reinterpret_cast<uint32_t*>(&v[j]);
+      const uint32_t uw[4] = {up[j].x, up[j].y, up[j].z, up[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 fg = unpack_bf16x2(g[i]), fu = unpack_bf16x2(uw[i]);
+        g[i] = pack_bf16x2(swiglu_row(fg.x, fu.x), swiglu_row(fg.y, fu.y));
       }
     }
   }
@@ -190,6 +211,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const T* __restrict__ x, long long ldx,
                                                                 int8_t* __restrict__ q, float* __restrict__ scale,
                                                                 int K, int Kp) {
+  pdl_launch_dependents();
   __shared__ uint32_t red_u[32];
   const long long row = blockIdx.x;
   const unsigned short* xr = reinterpret_cast<const unsigned short*>(x) + row * ldx;
@@ -246,12 +268,21 @@ struct Int8Params {
   int in_type;
   int bt, stages;                  // few tokens: tokens per tile, ring size
   int tiles_m, tiles_n, group_m;   // many tokens: the tile grid
+  int w_early;                     // weight loads need not wait for the kernel before
   int* status;
 };
 
 ACCERL_DEVINL int ld_cluster_s32(uint32_t addr) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+ACCERL_DEVINL int4 ld_cluster_s32x4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 ACCERL_DEVINL uint32_t pack_f16x2(float lo, float hi) {
@@ -270,13 +301,46 @@ ACCERL_DEVINL void store_from_float(void* p, long long i, int type, float v) {
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
+// Four neighbouring channels of a row: y = acc * sx * sw + bias (+ residual).
+template <int OUT>
+ACCERL_DEVINL void finish4(const Int8Params& p, long long t, int n, int4 acc, float sx, float4 sw, float4 b) {
+  float4 y = make_float4(__fmaf_rn(static_cast<float>(acc.x), sx * sw.x, b.x),
+                         __fmaf_rn(static_cast<float>(acc.y), sx * sw.y, b.y),
+                         __fmaf_rn(static_cast<float>(acc.z), sx * sw.z, b.z),
+                         __fmaf_rn(static_cast<float>(acc.w), sx * sw.w, b.w));
+  if (p.residual) {
+    const long long at = t * p.ldr + n;
+    if (p.in_type == kOutF32) {
+      const float4 r = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + at);
+      y.x += r.x, y.y += r.y, y.z += r.z, y.w += r.w;
+    } else {
+      const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p.residual) + at);
+      const bool bf = p.in_type == kOutBf16;
+      const float2 lo = bf ? Half16<__nv_bfloat16>::unpack(r.x) : Half16<__half>::unpack(r.x);
+      const float2 hi = bf ? Half16<__nv_bfloat16>::unpack(r.y) : Half16<__half>::unpack(r.y);
+      y.x += lo.x, y.y += lo.y, y.z += hi.x, y.w += hi.y;
+    }
+  }
+  const long long at = t * p.ldo + n;
+  if constexpr (OUT == kOutF32)
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = y;
+  else if constexpr (OUT == kOutBf16)
+    *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(p.out) + at) =
+        make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+  else
+    *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(p.out) + at) =
+        make_uint2(pack_f16x2(y.x, y.y), pack_f16x2(y.z, y.w));
+}
+
 // Few tokens: one tile of 128 output channels x bt tokens per cluster of CTAs. The weight rows are the MMA's
 // 128 rows, so a decode batch of few tokens wastes no tensor rows and streams the weight once. The CTAs of a
 // cluster split K (there are only N / 128 tiles to spread over 148 SMs): each leaves its integer partial in its
 // shared memory, and each sums and finishes its share of the tokens over the cluster. Integer sums have no
 // order, so the split changes no bit.
-//   warp 0: TMA producer into a ring of stages;  warp 1: TMEM and MMA issue;  warps 2-5: epilogue (one
-//   TMEM lane = one output channel per thread; the 32 lanes of a warp store 32 neighbouring channels).
+//   warp 0: TMA producer into a ring of stages;  warp 1: TMEM and MMA issue;  warps 2-5: accumulator to
+//   shared memory;  then all warps: a token row each, four neighbouring channels a lane (VEC: 16-byte rows) or
+//   every 32nd channel.
+template <int OUT, bool VEC>
 __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                       const __grid_constant__ CUtensorMap tmX,
                                                                       const Int8Params p) {
@@ -293,6 +357,8 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   const uint32_t stage_bytes = (kI8Rows + p.bt) * kI8BK;
   uint32_t cols = 32;
   while (cols < static_cast<uint32_t>(p.bt)) cols <<= 1;
+  bool ok = true;
+  int issued = 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
@@ -300,12 +366,20 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
     }
     mbar_init(&done, 1);
     fence_mbar_init();
+    // the first weight tiles start at once, behind a quantising kernel even before the tokens are there
+    // (p.w_early: nothing that kernel writes is part of the weight)
+    if (!p.w_early) pdl_wait();
+    for (; issued < min(p.stages, kbs); ++issued) {
+      mbar_arrive_expect_tx(&full[issued], stage_bytes);
+      tma_load_2d(smem + issued * stage_bytes, &tmW, &full[issued], (kb_first + issued) * kI8BK, n0);
+    }
+    pdl_wait();
+    for (int s = 0; s < issued; ++s)
+      tma_load_2d(smem + s * stage_bytes + kI8Rows * kI8BK, &tmX, &full[s], (kb_first + s) * kI8BK, t0);
   }
-  if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tmW);
-    prefetch_tmap(&tmX);
-  }
+  __syncwarp();
   if (warp == 1) tmem_alloc(&tmem_slot, cols);
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -313,9 +387,7 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
 
   if (warp == 0) {
     if (lane == 0) {
-      bool ok = true;
-      int issued = 0;
-      for (int kb = 0; kb < kbs; ++kb) {
+      for (int kb = issued; kb < kbs; ++kb) {
         const int s = kb % p.stages;
         if (!mbar_wait(&empty[s], ((kb / p.stages) & 1) ^ 1u, p.status, kStatusTimeoutProducer)) {
           ok = false;
@@ -334,7 +406,6 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = make_idesc_s8_s32(kI8Rows, p.bt);
-      bool ok = true;
       for (int kb = 0; kb < kbs; ++kb) {
         const int s = kb % p.stages;
         if (!mbar_wait(&full[s], (kb / p.stages) & 1, p.status, kStatusTimeoutMma)) {
@@ -352,42 +423,12 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
       }
       if (ok) umma_commit(&done);
     }
-  }
-  // this CTA's share of the tokens of the tile
-  const int share = (p.bt + splits - 1) / splits;
-  const int c_lo = split * share, c_hi = min(min(p.bt, p.M - t0), c_lo + share);
-  const int quarter = warp & 3;  // TMEM lanes this warp may read
-  const int n = n0 + quarter * 32 + lane;
-  const bool n_ok = warp >= 2 && n < p.N;
-  const float sw = n_ok ? p.sw[n] : 0.f;
-  const float b = (n_ok && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
-  auto finish = [&](int c, int acc) {
-    const long long t = t0 + c;
-    float y = static_cast<float>(acc) * (__ldg(p.sx + t) * sw) + b;
-    if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
-    store_from_float(p.out, t * p.ldo + n, p.out_type, y);
-  };
-  bool ok = false;
-  if (warp >= 2) {
-    ok = mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue);
-    tc_fence_after();
-    const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16);
-    if (splits == 1) {
-      if (ok) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < c_hi; c0 += 16) {
-          uint32_t v[16];
-          tmem_ld16(t_row + c0, v);
-          tmem_wait_ld();
-          if (n_ok) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c0 + i < c_hi) finish(c0 + i, static_cast<int>(v[i]));
-          }
-        }
-      }
-    } else if (ok) {
-      // every MMA of this CTA has read its stages: their memory takes the partial, [token][channel]
+  } else {
+    const int quarter = warp & 3;  // TMEM lanes this warp may read
+    if (mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue)) {
+      tc_fence_after();
+      const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16);
+      // every MMA of this CTA has read its stages: their memory takes the accumulator, [token][channel]
       int* part = reinterpret_cast<int*>(smem) + quarter * 32 + lane;
 #pragma unroll 1
       for (int c0 = 0; c0 < min(p.bt, p.M - t0); c0 += 16) {
@@ -400,25 +441,58 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
     }
     tc_fence_before();
   }
-  if (splits > 1) {
-    __syncthreads();
-    cluster_sync();
-    if (n_ok && ok) {
-      uint32_t base[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) base[r] = r < splits ? map_shared_rank(smem, r) + (quarter * 32 + lane) * 4 : 0u;
-      for (int c = c_lo; c < c_hi; ++c) {
-        int acc = 0;
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r < splits) acc += ld_cluster_s32(base[r] + c * (kI8Rows * 4));
-        finish(c, acc);
+  __syncthreads();
+  if (splits > 1) cluster_sync();
+
+  // this CTA's share of the tokens; a timed-out wait leaves what it finds there (the status word is set)
+  const int share = (p.bt + splits - 1) / splits;
+  const int c_lo = split * share, c_hi = min(min(p.bt, p.M - t0), c_lo + share);
+  constexpr int kWarps = kI8Threads / 32;
+  if constexpr (VEC) {
+    const int n = n0 + lane * 4;
+    if (n < p.N) {  // N is a multiple of 4
+      const float4 sw = *reinterpret_cast<const float4*>(p.sw + n);
+      float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p.bias)
+        b = make_float4(load_as_float(p.bias, n, p.in_type), load_as_float(p.bias, n + 1, p.in_type),
+                        load_as_float(p.bias, n + 2, p.in_type), load_as_float(p.bias, n + 3, p.in_type));
+#pragma unroll 2
+      for (int c = c_lo + warp; c < c_hi; c += kWarps) {
+        const uint32_t off = (c * kI8Rows + lane * 4) * 4;
+        int4 acc = *reinterpret_cast<const int4*>(smem + off);
+        for (int r = 1; r < splits; ++r) {
+          const int4 o = ld_cluster_s32x4(map_shared_rank(smem, (split + r) % splits) + off);
+          acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+        }
+        finish4<OUT>(p, t0 + c, n, acc, __ldg(p.sx + t0 + c), sw, b);
       }
     }
-    __syncthreads();
-    cluster_sync();  // nobody leaves while its partial may still be read
+  } else {
+    float sw[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + i * 32 + lane;
+      sw[i] = n < p.N ? p.sw[n] : 0.f;
+      b[i] = (n < p.N && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
+    }
+    for (int c = c_lo + warp; c < c_hi; c += kWarps) {
+      const long long t = t0 + c;
+      const float sx = __ldg(p.sx + t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + i * 32 + lane;
+        if (n >= p.N) continue;
+        const uint32_t off = (c * kI8Rows + i * 32 + lane) * 4;
+        int acc = *reinterpret_cast<const int*>(smem + off);
+        for (int r = 1; r < splits; ++r) acc += ld_cluster_s32(map_shared_rank(smem, (split + r) % splits) + off);
+        float y = __fmaf_rn(static_cast<float>(acc), sx * sw[i], b[i]);
+        if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
+        store_from_float(p.out, t * p.ldo + n, OUT, y);
+      }
+    }
   }
   __syncthreads();
+  if (splits > 1) cluster_sync();  // nobody leaves while its partial may still be read
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tbase, cols);
@@ -441,8 +515,10 @@ constexpr int kI8Tile = 256;    // tokens and channels per tile of a CTA pair
 constexpr int kI8Stages = 5;
 constexpr int kI8HalfBytes = 128 * kI8BK;          // a CTA's 128 rows of either operand
 constexpr int kI8StageBytes = 2 * kI8HalfBytes;
-constexpr int kI8EpiChunk = 32 * 128;              // 32 rows x 128 bytes per epilogue warp and buffer
-constexpr int kI8PairSmem = kI8Stages * kI8StageBytes + 4 * 2 * kI8EpiChunk + 2 * 2 * kI8Tile * 4 + 1024;
+constexpr int kI8EpiWarps = 8;                     // two per TMEM lane quarter, half of the channels each
+constexpr int kI8PairThreads = 64 + 32 * kI8EpiWarps;
+constexpr int kI8EpiBytes = 32 * 128;              // staging per epilogue warp: 32 rows x 32 columns of fp32
+constexpr int kI8PairSmem = kI8Stages * kI8StageBytes + kI8EpiWarps * kI8EpiBytes + 2 * 2 * kI8Tile * 4 + 1024;
 static_assert(kI8PairSmem + 1024 <= 232448, "shared memory per CTA");
 
 // tile t -> (token block, channel block), in groups of `group_m` token blocks for L2 reuse of the weight
@@ -456,19 +532,51 @@ ACCERL_DEVINL void int8_tile(const Int8Params& p, int t, int& m_blk, int& n_blk)
   n_blk = r / size;
 }
 
+// f[0..32) += residual[row, col0..col0 + 32), columns behind N left alone. Rows are 16-byte aligned.
+ACCERL_DEVINL void add_residual32(float (&f)[32], const Int8Params& p, long long row, int col0) {
+  const long long at = row * p.ldr + col0;
+  if (col0 + 32 > p.N) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (col0 + i < p.N) f[i] += load_as_float(p.residual, at + i, p.in_type);
+  } else if (p.in_type == kOutF32) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 r = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + at + i);
+      f[i] += r.x;
+      f[i + 1] += r.y;
+      f[i + 2] += r.z;
+      f[i + 3] += r.w;
+    }
+  } else {
+    const bool bf = p.in_type == kOutBf16;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      const uint4 r = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p.residual) + at + i);
+      const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = bf ? Half16<__nv_bfloat16>::unpack(rw[j]) : Half16<__half>::unpack(rw[j]);
+        f[i + 2 * j] += a.x;
+        f[i + 2 * j + 1] += a.y;
+      }
+    }
+  }
+}
+
 // The two CTAs of a pair compute one 256 x 256 tile with tcgen05.mma.cta_group::2: each stages its 128
 // tokens and 128 of the channels, the even CTA issues the MMAs, each drains the 128 x 256 accumulator of its
 // tokens. Accumulators are double-buffered in TMEM, so the epilogue of a tile runs under the next one's
 // products. TMA_OUT: the result leaves through swizzled shared memory and TMA stores (16-byte aligned rows);
 // otherwise, and for residuals that are not aligned, through fp32 staging and coalesced element stores.
 template <int OUT, bool TMA_OUT>
-__global__ void __launch_bounds__(kI8Threads, 1)
+__global__ void __launch_bounds__(kI8PairThreads, 1)
     gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                           const __grid_constant__ CUtensorMap tmOut, const Int8Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smEpi = smem + kI8Stages * kI8StageBytes;
-  float* sm_scale = reinterpret_cast<float*>(smEpi + 4 * 2 * kI8EpiChunk);  // [buffer][scale, bias][channel]
+  float* sm_scale = reinterpret_cast<float*>(smEpi + kI8EpiWarps * kI8EpiBytes);  // [buffer][scale, bias][channel]
   __shared__ uint64_t full[kI8Stages], empty[kI8Stages], tfull[2], tempty[2];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -482,7 +590,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 256);
+      mbar_init(&tempty[a], 2 * 32 * kI8EpiWarps);
     }
     fence_mbar_init();
   }
@@ -491,6 +599,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     prefetch_tmap(&tmW);
   }
   if (warp == 1) tmem_alloc_pair(&tmem_slot, 2 * kI8Tile);
+  pdl_wait();
   tc_fence_before();
   cluster_sync();  // barriers of both CTAs initialised before any remote signal
   tc_fence_after();
@@ -569,8 +678,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else {
     const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
     const uint32_t tempty_even = map_shared_rank(&tempty[0], 0);
-    uint8_t* wbuf = smEpi + quarter * (2 * kI8EpiChunk);
+    uint8_t* wbuf = smEpi + (warp - 2) * kI8EpiBytes;
     int local = 0, chunk = 0;
     for (int t = first; t < p.tiles_m * p.tiles_n; t += stride, ++local) {
       int m_blk, n_blk;
@@ -583,104 +693,86 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const float sx = row_ok ? __ldg(p.sx + row) : 0.f;
       // channel scales and bias of the tile, one buffer per accumulator
       float* scale = sm_scale + acc * 2 * kI8Tile;
-      for (int i = threadIdx.x - 64; i < kI8Tile; i += 128) {
+      for (int i = threadIdx.x - 64; i < kI8Tile; i += 32 * kI8EpiWarps) {
         const int n = n0 + i;
         scale[i] = n < p.N ? p.sw[n] : 0.f;
         scale[kI8Tile + i] = (n < p.N && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
       }
-      // the four warps go on, or give up, together
-      if (!named_bar_and(1, 128, mbar_wait(&tfull[acc], (local >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
+      // the epilogue warps go on, or give up, together
+      if (!named_bar_and(1, 32 * kI8EpiWarps, mbar_wait(&tfull[acc], (local >> 1) & 1, p.status, kStatusTimeoutEpilogue)))
+        break;
       tc_fence_after();
       const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kI8Tile;
-      constexpr int kCols = (TMA_OUT && OUT != kOutF32) ? 64 : 32;  // columns per 4 KB buffer
+      const int c_end = min(half * 128 + 128, p.N - n0);
+      uint32_t v[32];
+      if (half * 128 < c_end) tmem_ld32(t_row + half * 128, v);
 #pragma unroll 1
-      for (int c0 = 0; c0 < kI8Tile && n0 + c0 < p.N; c0 += kCols) {
-        uint8_t* buf = wbuf + (chunk & 1) * kI8EpiChunk;
-        ++chunk;
-        if constexpr (TMA_OUT) {
-          if (lane == 0) bulk_wait_read<1>();  // the store issued from this buffer two chunks ago
-        }
-        __syncwarp();
-        uint32_t v[kCols];
-#pragma unroll
-        for (int h = 0; h < kCols; h += 32) tmem_ld32(t_row + c0 + h, *reinterpret_cast<uint32_t(*)[32]>(v + h));
+      for (int c0 = half * 128; c0 < c_end; c0 += 32) {
         tmem_wait_ld();
+        float f[32];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {  // 16-byte pieces of the staged row
-          constexpr int kPer = kCols / 8;
-          float f[kPer];
+        for (int i = 0; i < 32; ++i) f[i] = static_cast<float>(static_cast<int>(v[i]));
+        if (c0 + 32 < c_end) tmem_ld32(t_row + c0 + 32, v);  // the next columns travel while these are finished
 #pragma unroll
-          for (int i = 0; i < kPer; i += 4) {
-            const int c = c0 + j * kPer + i;
-            const float4 s4 = *reinterpret_cast<const float4*>(scale + c);
-            const float4 b4 = *reinterpret_cast<const float4*>(scale + kI8Tile + c);
-            f[i] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i])), sx * s4.x, b4.x);
-            f[i + 1] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i + 1])), sx * s4.y, b4.y);
-            f[i + 2] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i + 2])), sx * s4.z, b4.z);
-            f[i + 3] = __fmaf_rn(static_cast<float>(static_cast<int>(v[j * kPer + i + 3])), sx * s4.w, b4.w);
+        for (int i = 0; i < 32; i += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(scale + c0 + i);
+          const float4 b4 = *reinterpret_cast<const float4*>(scale + kI8Tile + c0 + i);
+          f[i] = __fmaf_rn(f[i], sx * s4.x, b4.x);
+          f[i + 1] = __fmaf_rn(f[i + 1], sx * s4.y, b4.y);
+          f[i + 2] = __fmaf_rn(f[i + 2], sx * s4.z, b4.z);
+          f[i + 3] = __fmaf_rn(f[i + 3], sx * s4.w, b4.w);
+        }
+        const int col0 = n0 + c0;
+        if constexpr (TMA_OUT) {
+          if (p.residual && row_ok) add_residual32(f, p, row, col0);
+          // 16-bit results: two buffers of 32 rows x 64 bytes; fp32: one of 32 x 128
+          uint8_t* buf = wbuf + (OUT == kOutF32 ? 0 : (chunk & 1) * (kI8EpiBytes / 2));
+          ++chunk;
+          if (lane == 0) {  // the store issued from this buffer has read it
+            if constexpr (OUT == kOutF32) bulk_wait_read<0>();
+            else bulk_wait_read<1>();
           }
-          if constexpr (TMA_OUT) {
-            if (p.residual && row_ok) {
-              // aligned rows: whole pieces lie inside the row's allocation when their first column does
-              const int col = n0 + c0 + j * kPer;
-              const long long at = row * p.ldr + col;
-              if (col + kPer <= p.N) {
-                if (p.in_type == kOutF32) {
+          __syncwarp();
+          if constexpr (OUT == kOutF32) {
 #pragma unroll
-                  for (int i = 0; i < kPer; i += 4) {
-                    const float4 r = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + at + i);
-                    f[i] += r.x;
-                    f[i + 1] += r.y;
-                    f[i + 2] += r.z;
-                    f[i + 3] += r.w;
-                  }
-                } else {
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(buf + swz128(lane, j)) =
+                  make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+          } else {
 #pragma unroll
-                  for (int i = 0; i < kPer; i += 4) {
-                    const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p.residual) + at + i);
-                    const float2 a = p.in_type == kOutBf16 ? Half16<__nv_bfloat16>::unpack(r.x) : Half16<__half>::unpack(r.x);
-                    const float2 b = p.in_type == kOutBf16 ? Half16<__nv_bfloat16>::unpack(r.y) : Half16<__half>::unpack(r.y);
-                    f[i] += a.x;
-                    f[i + 1] += a.y;
-                    f[i + 2] += b.x;
-                    f[i + 3] += b.y;
-                  }
-                }
-              } else {
+            for (int j = 0; j < 4; ++j) {
+              uint32_t o[4];
 #pragma unroll
-                for (int i = 0; i < kPer; ++i)
-                  if (col + i < p.N) f[i] += load_as_float(p.residual, at + i, p.in_type);
-              }
+              for (int i = 0; i < 4; ++i)
+                o[i] = OUT == kOutBf16 ? pack_bf16x2(f[8 * j + 2 * i], f[8 * j + 2 * i + 1])
+                                       : pack_f16x2(f[8 * j + 2 * i], f[8 * j + 2 * i + 1]);
+              *reinterpret_cast<uint4*>(buf + swz64(lane, j)) = make_uint4(o[0], o[1], o[2], o[3]);
             }
           }
-          uint4 o;
-          if constexpr (TMA_OUT && OUT == kOutBf16)
-            o = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-          else if constexpr (TMA_OUT && OUT == kOutF16)
-            o = make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
-          else
-            o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-          *reinterpret_cast<uint4*>(buf + swz128(lane, j)) = o;
-        }
-        if constexpr (TMA_OUT) {
           fence_async_shared();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmOut, buf, n0 + c0, y0);
+            tma_store_2d(&tmOut, buf, col0, y0);
             bulk_commit();
           }
         } else {
           __syncwarp();
-          const int n = n0 + c0 + lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(wbuf + swz128(lane, j)) =
+                make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+          __syncwarp();
+          const int n = col0 + lane;
           if (n < p.N) {
-            for (int r = 0; r < 32 && y0 + r < p.M; ++r) {
-              float y = *reinterpret_cast<const float*>(buf + swz128(r, lane >> 2) + (lane & 3) * 4);
+            const int rows = min(32, p.M - y0);
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r) {
+              float y = *reinterpret_cast<const float*>(wbuf + swz128(r, lane >> 2) + (lane & 3) * 4);
               const long long at = y0 + r;
               if (p.residual) y += load_as_float(p.residual, at * p.ldr + n, p.in_type);
               store_from_float(p.out, at * p.ldo + n, OUT, y);
             }
           }
-          __syncwarp();
         }
       }
       tc_fence_before();
@@ -728,7 +820,7 @@ bool make_int8_map(CUtensorMap* out, const void* ptr, uint64_t pitch, uint64_t r
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Map of the output for tiles of 128 bytes x 32 rows. False when TMA cannot store it (alignment).
+// Map of the output for tiles of 32 columns x 32 rows. False when TMA cannot store it (alignment).
 bool make_out_map(CUtensorMap* out, const Int8Params& p) {
   const uint64_t es = p.out_type == kOutF32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(p.out) & 15) || (p.ldo * es) % 16 || p.ldo < p.N) return false;
@@ -736,27 +828,31 @@ bool make_out_map(CUtensorMap* out, const Int8Params& p) {
   if (!fn) return false;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.N), static_cast<cuuint64_t>(p.M)};
   cuuint64_t strides[1] = {p.ldo * es};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), 32};
+  cuuint32_t box[2] = {32, 32};
   cuuint32_t estr[2] = {1, 1};
   const CUtensorMapDataType dt = p.out_type == kOutF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : p.out_type == kOutF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return fn(out, dt, 2, p.out, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return fn(out, dt, 2, p.out, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-cudaLaunchConfig_t cluster_config(dim3 grid, int smem, cudaStream_t s, cudaLaunchAttribute* attr, unsigned x, unsigned z) {
+cudaLaunchConfig_t cluster_config(dim3 grid, int threads, int smem, cudaStream_t s, cudaLaunchAttribute* attr, unsigned x,
+                                  unsigned z) {
   cudaLaunchConfig_t cfg = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = x;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = z;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kI8Threads, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cfg;
 }
 
@@ -766,20 +862,30 @@ int launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap&
   static std::atomic<int> cache[kMaxHostDevices];  // pairs that can be resident at once, per device
   const int dev = host_current_device();
   if (dev < 0 || dev >= kMaxHostDevices) return -14;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   int pairs = cache[dev].load(std::memory_order_acquire);
   if (pairs == 0) {
     cudaError_t e = smem_attr_once<gemm_int8_pair_kernel<OUT, TMA_OUT>>(kI8PairSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
-    cudaLaunchConfig_t cfg = cluster_config(dim3(2 * (device_sm_count() / 2)), kI8PairSmem, s, attr, 2, 1);
+    cudaLaunchConfig_t cfg = cluster_config(dim3(2 * (device_sm_count() / 2)), kI8PairThreads, kI8PairSmem, s, attr, 2, 1);
+    cfg.numAttrs = 1;
     e = cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (pairs < 1) return -13;
     cache[dev].store(pairs, std::memory_order_release);
   }
   const int grid = 2 * std::min(pairs, p.tiles_m * p.tiles_n);
-  cudaLaunchConfig_t cfg = cluster_config(dim3(grid), kI8PairSmem, s, attr, 2, 1);
+  cudaLaunchConfig_t cfg = cluster_config(dim3(grid), kI8PairThreads, kI8PairSmem, s, attr, 2, 1);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, mx, mw, mo, p));
+}
+
+template <int OUT, bool VEC>
+int launch_stream(const CUtensorMap& mw, const CUtensorMap& mx, const Int8Params& p, dim3 grid, int smem, cudaStream_t s) {
+  cudaError_t e = smem_attr_once<gemm_int8_stream_kernel<OUT, VEC>>(201 * 1024);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = cluster_config(grid, kI8Threads, smem, s, attr, 1, grid.z);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_stream_kernel<OUT, VEC>, mw, mx, p));
 }
 
 template <typename T, int PRE>
@@ -796,14 +902,18 @@ int launch_quantize(const T* x, long long ldx, const T* w, float eps, int8_t* q,
       return -2;
     }
   }
+  // the fewest threads a row that hold it in 4 chunks each (SwiGLU: of both halves), 512 at most
   int tpr = 32;
-  while (tpr < 1024 && chunks > 4 * tpr) tpr *= 2;
+  while (tpr < 512 && chunks > 4 * tpr) tpr *= 2;
   const int block = std::max(tpr, 128);
   const int nc = (chunks + tpr - 1) / tpr;
   const unsigned grid = static_cast<unsigned>((rows + block / tpr - 1) / (block / tpr));
-  if (nc <= 1) quantize_rows_kernel<T, PRE, 1><<<grid, block, 0, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, tpr);
-  else if (nc <= 2) quantize_rows_kernel<T, PRE, 2><<<grid, block, 0, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, tpr);
-  else quantize_rows_kernel<T, PRE, 4><<<grid, block, 0, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, tpr);
+  auto launch = [&](auto kern) { kern<<<grid, block, 0, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, tpr); };
+  if (nc <= 1) launch(quantize_rows_kernel<T, PRE, 1>);
+  else if (nc <= 2) launch(quantize_rows_kernel<T, PRE, 2>);
+  else if (nc <= 3) launch(quantize_rows_kernel<T, PRE, 3>);
+  else if (nc <= 4) launch(quantize_rows_kernel<T, PRE, 4>);
+  else launch(quantize_rows_kernel<T, PRE, 8>);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -833,10 +943,11 @@ extern "C" int accerl_quantize_rows(const void* x, long long ldx, int half, int 
 }
 
 // out [M, N] (out_type) = sx sw (qx qw^T) (+ bias [N]) (+ residual [M, N]), bias and residual of in_type
-// (types: 0 bf16, 1 fp16, 2 fp32). qx [M, Kp] and qw [N, Kp], Kp = K rounded up to 16.
+// (types: 0 bf16, 1 fp16, 2 fp32). qx [M, Kp] and qw [N, Kp], Kp = K rounded up to 16. `w_early`: the kernel
+// before this one on the stream writes nothing of the weight, so its loads need not wait for that kernel.
 extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw, const float* sw, int M, int N, int K,
                                 const void* bias, const void* residual, long long ldr, int in_type, void* out,
-                                long long ldo, int out_type, int* status, cudaStream_t stream) {
+                                long long ldo, int out_type, int w_early, int* status, cudaStream_t stream) {
   using namespace accerl;
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 133144) return -1;
@@ -856,6 +967,7 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   p.out_type = out_type;
   p.in_type = in_type;
   p.status = status;
+  p.w_early = w_early;
   p.tiles_m = (M + kI8Tile - 1) / kI8Tile;
   p.tiles_n = (N + kI8Tile - 1) / kI8Tile;
   p.group_m = 8;
@@ -885,15 +997,17 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   const int stage_bytes = (kI8Rows + p.bt) * kI8BK;
   const int budget = tiles * splits > device_sm_count() ? 100 * 1024 : 200 * 1024;
   p.stages = std::max(2, std::min({16, (kbs + splits - 1) / splits, budget / stage_bytes}));
-  int smem_bytes = p.stages * stage_bytes;
-  if (splits > 1) smem_bytes = std::max(smem_bytes, p.bt * kI8Rows * 4);  // the partial
-  smem_bytes += 1024;
+  // the accumulator in the end lies where the stages were
+  const int smem_bytes = std::max(p.stages * stage_bytes, p.bt * kI8Rows * 4) + 1024;
   CUtensorMap mw, mx;
   if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), kI8Rows)) return -7;
   if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), static_cast<uint32_t>(p.bt))) return -8;
-  cudaError_t e = smem_attr_once<gemm_int8_stream_kernel>(201 * 1024);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = cluster_config(dim3(tiles, 1, splits), smem_bytes, stream, attr, 1, splits);
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_stream_kernel, mw, mx, p));
+  const int es = out_type == kOutF32 ? 4 : 2, rs = in_type == kOutF32 ? 4 : 2;
+  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * es) % (4 * es) == 0 &&
+                   (reinterpret_cast<uintptr_t>(sw) & 15) == 0 &&
+                   (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * rs) % (4 * rs) == 0));
+  const dim3 grid(tiles, 1, splits);
+  if (out_type == kOutBf16) return vec ? launch_stream<kOutBf16, true>(mw, mx, p, grid, smem_bytes, stream) : launch_stream<kOutBf16, false>(mw, mx, p, grid, smem_bytes, stream);
+  if (out_type == kOutF16) return vec ? launch_stream<kOutF16, true>(mw, mx, p, grid, smem_bytes, stream) : launch_stream<kOutF16, false>(mw, mx, p, grid, smem_bytes, stream);
+  return vec ? launch_stream<kOutF32, true>(mw, mx, p, grid, smem_bytes, stream) : launch_stream<kOutF32, false>(mw, mx, p, grid, smem_bytes, stream);
 }
