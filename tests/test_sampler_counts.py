@@ -180,6 +180,31 @@ def test_masked_and_special_logits(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v", [70, 9001])
+def test_values_outside_the_usual_range(device, dtype, v):
+    """Rows with logits that are tiny, huge, or masked with low numbers that do or do not weigh something:
+    the kernel counts such values apart."""
+    x, u, g = make(10, v, device, dtype, seed=11)
+    x[0, 3] = 1e-13 if dtype == torch.bfloat16 else 90.0
+    x[1] *= 1e-14 if dtype == torch.bfloat16 else 20.0
+    x[2, ::2] = torch.finfo(dtype).min
+    x[3, 1:] = torch.finfo(dtype).min
+    x[4] = torch.finfo(dtype).min
+    x[5, ::3] = -1e4
+    x[6, ::5] = -70.0
+    x[7, 5:9] = torch.finfo(dtype).max
+    x[8, v // 2:] = float("inf")
+    x[9, ::4] = -x[9].abs().max()
+    t = full(10, 1.0, device)
+    check(x, u, t)
+    check(x, u, full(10, 300.0, device))  # -1e4 and -70 weigh something
+    check(x, u, full(10, 1e5, device), full(10, v - 3, device, torch.int32))
+    check(x, u, full(10, 0.7, device), full(10, 30, device, torch.int32), full(10, 0.9, device), full(10, 0.01, device))
+    check(x, u, full(10, 0.0, device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_numbers_outside_their_range(device):
     x, _, _ = make(1, 300, device, torch.bfloat16)
     x = x.expand(6, -1)
