@@ -10,11 +10,10 @@
 // tokens of that value; a second look at the row (from L2) finds that token. There is no sort, one 64-bit
 // exponential per value that occurs, and only integer atomics, so a result does not depend on their order.
 //
-// Counters for all values would fill 128 KB and leave one block to an SM, whose counting then waits for its own
-// searches and barriers. So the kernel counts a window of the values that logits take (bf16: zero and 2^-40 to
-// 2^24; fp16: below 64, each sign) in 32 KB (84 KB). Lower values, masks of the type's lowest value among them, are
-// left out where they weigh nothing; a row with any other value takes the slow path, which counts all values,
-// window by window.
+// Counters for all values would not fit an SM. The kernel counts a window of the values that logits take (bf16: zero
+// and 2^-40 to 2^24; fp16: below 64, each sign) in 64 KB (168 KB). Lower values, masks of the type's lowest value
+// among them, are left out where they weigh nothing; a row with any other value takes the slow path, which counts
+// all values, window by window.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -24,46 +23,99 @@
 namespace accerl {
 
 constexpr int kCntGroups = 1024;              // at most: groups of 64 neighbouring values
-constexpr int kCntMaxSlice = 65528;           // elements a CTA may count without overflowing 16 bits
 constexpr int kCntMaxCluster = 8;
 // tokens further below the largest logit than this many temperatures weigh nothing: all of a row's together
 // hold less than 1e-20 of its mass, far below what a 64-bit sum resolves
 constexpr double kCntNegligible = 60.0;
 
-// Order-preserving 16-bit keys of the finite values and +inf: (kNegInf, kPosInf]. The window holds kP
-// magnitudes of each sign from the pattern kLo on; the slot of kLo itself is that of zero.
+// Order-preserving 16-bit keys of the finite values and +inf: (kNegInf, kPosInf].
+// The window holds kSlots magnitude patterns from kBase on (fp16: without the first, zero). Its bins ascend with
+// the value: [64, 64 + kSlots) negative, then as many positive ones; bin 0, whose group of 64 has no other use, is
+// zero's. kBase and kSlots are multiples of 4, so four neighbouring bins from a multiple of 4 on are evenly spaced.
 template <typename T>
 struct Key16;
 template <>
 struct Key16<__nv_bfloat16> {
   static constexpr uint32_t kInf = 0x7f80u, kPosInf = 0xff80u, kNegInf = 0x007fu;
-  static constexpr uint32_t kLo = ((127u - 40u) << 7) - 1u, kP = 64u << 7;
-  static constexpr int kBlocksPerSm = 4;
+  static constexpr uint32_t kBase = (127u - 40u) << 7, kSlots = 64u << 7, kMantissa = 7;
+  static constexpr bool kOneRow = false;  // the counters leave room for two blocks on an SM
   static ACCERL_DEVINL float value(uint32_t bits) { return __uint_as_float(bits << 16); }
+  static ACCERL_DEVINL uint32_t max2(uint32_t a, uint32_t b) {  // of both halves; a NaN loses
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  // n += elements of the 8 words' halves equal to the value in both halves of `want` (0 equals -0, NaN nothing)
+  static ACCERL_DEVINL void count_equal(const uint4 (&v)[8], uint32_t want, uint32_t& n) {
+    const __nv_bfloat162 k = *reinterpret_cast<__nv_bfloat162*>(&want);
+    __nv_bfloat162 sum = __float2bfloat162_rn(0.f);  // at most 32 a half: exact
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = __hadd2(sum, __heq2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), k));
+    }
+    n += static_cast<uint32_t>(__low2float(sum) + __high2float(sum));
+  }
+  // halves that are not 0 where w, whose magnitude is t - 0x8000 + kBase, is not in the window
+  static ACCERL_DEVINL uint32_t outside(uint32_t w, uint32_t t) { return (t & 0xe000e000u) ^ 0x80008000u; }
 };
 template <>
 struct Key16<__half> {
   static constexpr uint32_t kInf = 0x7c00u, kPosInf = 0xfc00u, kNegInf = 0x03ffu;
-  static constexpr uint32_t kLo = 0u, kP = 21u << 10;
-  static constexpr int kBlocksPerSm = 2;
+  static constexpr uint32_t kBase = 0u, kSlots = 21u << 10, kMantissa = 10;
+  static constexpr bool kOneRow = true;
   static ACCERL_DEVINL float value(uint32_t bits) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
   }
+  static ACCERL_DEVINL uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  static ACCERL_DEVINL void count_equal(const uint4 (&v)[8], uint32_t want, uint32_t& n) {
+    const __half2 k = *reinterpret_cast<__half2*>(&want);
+    __half2 sum = __float2half2_rn(0.f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = __hadd2(sum, __heq2(*reinterpret_cast<const __half2*>(&w[i]), k));
+    }
+    n += static_cast<uint32_t>(__low2float(sum) + __high2float(sum));
+  }
+  static ACCERL_DEVINL uint32_t outside(uint32_t w, uint32_t t) {
+    return (~(t - 0x00010001u) | ((w & 0x7fff7fffu) + (0x8000u - kSlots) * 0x00010001u)) & 0x80008000u;
+  }
 };
+// 0xffff in each half whose top bit is set
+ACCERL_DEVINL uint32_t half_masks(uint32_t v) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(r) : "r"(v));
+  return r;
+}
 ACCERL_DEVINL uint32_t key_bits(uint32_t key) { return (key & 0x8000u) ? key ^ 0x8000u : key ^ 0xffffu; }
 ACCERL_DEVINL uint32_t bits_key(uint32_t bits) { return (bits & 0x8000u) ? bits ^ 0xffffu : bits ^ 0x8000u; }
-// window bin (ascending with the value) <-> key
 template <typename T>
 ACCERL_DEVINL uint32_t bin_key(uint32_t b) {
-  constexpr uint32_t P = Key16<T>::kP, lo = Key16<T>::kLo;
-  if (b == P) return 0x8000u;
-  return b > P ? 0x8000u + lo + (b - P) : 0x7fffu - lo - (P - 1 - b);
+  constexpr uint32_t S = Key16<T>::kSlots, base = Key16<T>::kBase;
+  if (b < 64u) return 0x8000u;
+  return b >= 64u + S ? 0x8000u + base + (b - 64u - S) : 0x7fffu - base - (63u + S - b);
 }
 template <typename T>
 ACCERL_DEVINL uint32_t key_bin(uint32_t key) {
-  constexpr uint32_t P = Key16<T>::kP, lo = Key16<T>::kLo;
-  if (key == 0x8000u) return P;
-  return key > 0x8000u ? key - 0x8000u - lo + P : key + lo + P - 0x8000u;
+  constexpr uint32_t S = Key16<T>::kSlots, base = Key16<T>::kBase;
+  if (key == 0x8000u) return 0u;
+  return key > 0x8000u ? key - 0x8000u - base + 64u + S : key + base + 64u + S - 0x8000u;
+}
+// Group p (bins 64 p ..) of the window in descending order of its values: positive, zero, negative; and back.
+template <typename T>
+ACCERL_DEVINL int window_order(int p) {
+  constexpr int half = static_cast<int>(Key16<T>::kSlots / 64);
+  return p == 0 ? half : (p > half ? 2 * half - p : 2 * half + 1 - p);
+}
+template <typename T>
+ACCERL_DEVINL int window_group(int g) {
+  constexpr int half = static_cast<int>(Key16<T>::kSlots / 64);
+  return g == half ? 0 : (g < half ? 2 * half - g : 2 * half + 1 - g);
 }
 
 ACCERL_DEVINL double warp_scan_f64(double v, int lane) {  // inclusive
@@ -96,7 +148,8 @@ struct CountShared {
   uint32_t warp_u[3][32];
   double warp_d[32];
   double exp2_table[64];            // 2^(j / 64)
-  uint32_t max_in, max_low, max_all, escape;  // of this CTA's slice
+  double ratio[2][64];              // of neighbouring values' masses by binade of the window: at T, at 1
+  uint32_t max_key, max_low, escape;          // of this CTA's slice: keys, and whether a value escapes the window
   uint32_t group_cnt[64];                     // slow path: tokens of a group's values
   int found;                                  // a search's group
   uint32_t key, nth;                          // its value and rank among the value's tokens
@@ -104,6 +157,9 @@ struct CountShared {
   int nth_here;                               // rank of the drawn token within this CTA's slice, or -1
   float logprob;
 };
+
+// a count as a 64-bit float without the slow conversion
+ACCERL_DEVINL double count_f64(uint32_t n) { return __hiloint2double(0x43300000, static_cast<int>(n)) - 0x1p52; }
 
 // 2^(y / 64) for y <= 0: n = round(y), the table for n mod 64, and the Taylor series of the rest, |r| <= ln 2 / 128,
 // whose sixth term is below 2^-54. The argument's rounding costs at most a relative |y| 2^-59, so a weight is
@@ -141,20 +197,33 @@ struct RowWeights {
   }
   ACCERL_DEVINL double weight(uint32_t key) const { return mass(key, scale); }
   ACCERL_DEVINL double plain(uint32_t key) const { return mass(key, kLog2e64); }  // exp(x - max)
+  // masses of four neighbouring keys, ascending; `even`: equally spaced and none above the maximum, so that
+  // each is the one above it times the ratio r
+  ACCERL_DEVINL void mass4(const uint32_t (&key)[4], bool even, double r, double sc, double (&w)[4]) const {
+    if (even) {
+      w[3] = mass(key[3], sc);
+      w[2] = w[3] * r;
+      w[1] = w[2] * r;
+      w[0] = w[1] * r;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = mass(key[j], sc);
+    }
+  }
   ACCERL_DEVINL bool kept(uint32_t key, double w) const { return key == max_key || !(min_p > 0.0) || w >= min_p; }
 };
 
 // One row per cluster of CTAs, each counting a slice of it.
 template <typename T, int kCntThreads>
-__global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T>::kBlocksPerSm)
+__global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     sample_counts_kernel(const T* __restrict__ logits, long long ld, int V, const float* __restrict__ u,
                          const float* __restrict__ temperature, const int* __restrict__ top_k,
                          const float* __restrict__ top_p, const float* __restrict__ min_p,
                          long long* __restrict__ out_tokens, float* __restrict__ out_logprobs, int csize) {
-  constexpr uint32_t P = Key16<T>::kP, kBins = 2 * P;
+  constexpr uint32_t S = Key16<T>::kSlots, kBins = 64 + 2 * S;
   constexpr int kCntWarps = kCntThreads / 32, kCntPer = kCntGroups / kCntThreads;
   extern __shared__ uint4 dyn[];
-  uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);  // kBins 16-bit counters, two to a word
+  uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);  // kBins counters and 64 more that stay zero
   __shared__ CountShared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -178,75 +247,106 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  // f(bits) for every element of the chunks [a, b)
+  // f(word) for every two elements of the chunks [a, b). Whole chunks are loaded without a branch, several in
+  // flight a thread; the one or two at the row's ends that are not whole are one thread's.
+  const int whole0 = head ? 1 : 0, whole1 = (head + V) / 8;
+  const uint4* src = reinterpret_cast<const uint4*>(x - head);
   auto for_each = [&](int a, int b, auto f) {
     constexpr int kAhead = 4;
-    for (int c = a + tid; c < b; c += kCntThreads * kAhead) {
+    const int a1 = max(a, whole0), b1 = min(b, whole1);
+    auto words = [&](uint4 v) {
+      f(v.x);
+      f(v.y);
+      f(v.z);
+      f(v.w);
+    };
+    int c = a1 + tid;
+    for (; c + (kAhead - 1) * kCntThreads < b1; c += kCntThreads * kAhead) {
       uint4 v[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        v[j] = c + j * kCntThreads < b ? load8(c + j * kCntThreads) : make_uint4(~0u, ~0u, ~0u, ~0u);
+      for (int j = 0; j < kAhead; ++j) v[j] = __ldg(src + c + j * kCntThreads);
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const uint32_t vw[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f(vw[i] & 0xffffu);
-          f(vw[i] >> 16);
-        }
-      }
+      for (int j = 0; j < kAhead; ++j) words(v[j]);
+    }
+    for (; c < b1; c += kCntThreads) words(__ldg(src + c));
+    if (tid == 0) {
+      if (a < whole0 && a < b) words(load8(a));
+      if (b > whole1 && whole1 >= max(a, whole0)) words(load8(whole1));
     }
   };
-  auto clear = [&]() {
-    for (int i = tid; i < static_cast<int>(kBins / 8); i += kCntThreads) dyn[i] = make_uint4(0, 0, 0, 0);
+  auto valid_key = [](uint32_t w) -> int {  // -1: -inf or NaN
+    const uint32_t bits = w & 0xffffu, key = bits_key(bits == 0x8000u ? 0u : bits);
+    return key > Key16<T>::kNegInf && key <= Key16<T>::kPosInf ? static_cast<int>(key) : -1;
   };
-  auto add = [&](uint32_t bin) { atomicAdd(&hist[bin >> 1], 1u << ((bin & 1u) * 16)); };
+  auto clear = [&]() {
+    for (int i = tid; i < static_cast<int>((kBins + 64) / 4); i += kCntThreads) dyn[i] = make_uint4(0, 0, 0, 0);
+  };
+  auto add = [&](uint32_t bin) { atomicAdd(&hist[bin], 1u); };
 
+  // the row's settings, on their way while the slice is counted
+  const float t = temperature[row], row_u = u[row];
+  const float row_p = top_p ? top_p[row] : 1.f, row_min = min_p ? min_p[row] : 0.f;
+  const int row_k = top_k ? top_k[row] : 0;
   clear();
   if (tid == 0) sh.nth_here = -1;
+  const bool greedy = !(t > 0.f);
+  const double td = greedy ? 1.0 : static_cast<double>(t);
   if (tid < 64) sh.exp2_table[tid] = exp2(tid / 64.0);
+  if (tid >= 64 && tid < 192 && ((tid - 64) & 63) < static_cast<int>(S >> Key16<T>::kMantissa)) {
+    const uint32_t first = Key16<T>::kBase + (((tid - 64) & 63) << Key16<T>::kMantissa);
+    const double step = static_cast<double>(Key16<T>::value(first + 1) - Key16<T>::value(first));
+    sh.ratio[(tid - 64) >> 6][(tid - 64) & 63] = exp(-step / (tid < 128 ? td : 1.0));
+  }
   __syncthreads();
 
   // ---- count the slice ----
-  uint32_t max_in = 0, max_low = 0, max_all = 0, escape = 0;
-  for_each(ch0, ch1, [&](uint32_t bits) {
-    const uint32_t mag = bits & 0x7fffu, slot = mag - Key16<T>::kLo;
-    const uint32_t neg = (bits & 0x8000u) ? ~0u : 0u;
-    if (slot - 1u < P - 1u) {
-      const uint32_t bin = P + (slot ^ neg);
-      max_in = max(max_in, bin + 1u);
-      add(bin);
-    } else if (mag == 0u) {
-      max_in = max(max_in, P + 1u);
-      add(P);
-    } else if (mag < Key16<T>::kInf || bits == Key16<T>::kInf) {  // outside the window; -inf and NaN are nothing
-      const uint32_t key = bits_key(bits);
-      max_all = max(max_all, key);
-      if (neg && mag >= Key16<T>::kLo + P) max_low = max(max_low, key);
-      else escape = 1u;
+  uint32_t max2 = 0xffffffffu, max_low = 0, escape = 0;  // NaN: loses to everything
+  for_each(ch0, ch1, [&](uint32_t w) {
+    // Both halves at once, with plain 32-bit operations (the integer pipe is what bounds this loop): no sum of a
+    // half carries or borrows. With slot = magnitude - kBase, t = 0x8000 + slot, its complement for a negative value
+    // is 0x7fff - slot, and v - (0x8000 - 64 - kSlots) is the bin of either sign.
+    constexpr uint32_t kOnes = 0x00010001u, kOff = 0x8000u - 64u - S;
+    max2 = Key16<T>::max2(max2, w);
+    const uint32_t t = (w | 0x80008000u) - Key16<T>::kBase * kOnes, v = t ^ half_masks(w);
+    const uint32_t out = Key16<T>::outside(w, t);
+    if (!(out & 0xffffu)) add((v & 0xffffu) - kOff);
+    if (!(out >> 16)) add((v >> 16) - kOff);
+    // zeros and finite values outside the window; infinities and NaN have the top bit of `special` (+inf shows in
+    // max2, the others are nothing)
+    const uint32_t special = (w & 0x7fff7fffu) + (0x8000u - Key16<T>::kInf) * kOnes;
+    const uint32_t odd = (out & 0xffffu && !(special & 0x8000u) ? 1u : 0u) | (out >> 16 && !(special >> 31) ? 2u : 0u);
+    if (odd) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!(odd & (1u << h))) continue;
+        const uint32_t bits = (w >> (16 * h)) & 0xffffu, m = bits & 0x7fffu;
+        if (m == 0u) add(0u);
+        else if (m >= Key16<T>::kBase + S && bits != m) max_low = max(max_low, bits_key(bits));
+        else escape = 1u;
+      }
     }
   });
-  max_in = __reduce_max_sync(0xffffffffu, max_in);
+  max2 = Key16<T>::max2(max2, max2 >> 16 | max2 << 16) & 0xffffu;
+  uint32_t max_key = (max2 & 0x7fffu) > Key16<T>::kInf ? 0u : bits_key((max2 & 0x7fffu) ? max2 : 0u);
+  if (max_key <= Key16<T>::kNegInf) max_key = 0u;
+  if (max_key == Key16<T>::kPosInf) escape = 1u;
+  max_key = __reduce_max_sync(0xffffffffu, max_key);
   max_low = __reduce_max_sync(0xffffffffu, max_low);
-  max_all = __reduce_max_sync(0xffffffffu, max_all);
   escape = __reduce_max_sync(0xffffffffu, escape);
   if (lane == 0) {
-    sh.warp_u[0][warp] = max_in;
+    sh.warp_u[0][warp] = max_key;
     sh.warp_u[1][warp] = max_low;
-    sh.warp_u[2][warp] = (max_all << 1) | escape;
+    sh.warp_u[2][warp] = escape;
   }
   __syncthreads();
   if (warp == 0) {
     const bool has = lane < kCntWarps;
-    const uint32_t all = has ? sh.warp_u[2][lane] : 0u;
-    max_in = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[0][lane] : 0u);
+    max_key = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[0][lane] : 0u);
     max_low = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[1][lane] : 0u);
-    max_all = __reduce_max_sync(0xffffffffu, all >> 1);
-    escape = __reduce_max_sync(0xffffffffu, all & 1u);
+    escape = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[2][lane] : 0u);
     if (lane == 0) {
-      sh.max_in = max_in;
+      sh.max_key = max_key;
       sh.max_low = max_low;
-      sh.max_all = max_all;
       sh.escape = escape;
     }
   }
@@ -254,48 +354,39 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
   cluster_sync();
 
   // ---- the row's largest value, and whether the window holds all that matters ----
-  max_in = max_low = max_all = escape = 0;
+  max_key = max_low = escape = 0;
 #pragma unroll
   for (int c = 0; c < kCntMaxCluster; ++c)
     if (c < csize) {
       const CountShared* o = peer(&sh, c);
-      max_in = max(max_in, o->max_in);
+      max_key = max(max_key, o->max_key);
       max_low = max(max_low, o->max_low);
-      max_all = max(max_all, o->max_all);
       escape |= o->escape;
     }
   RowWeights<T> rw;
-  const float t = temperature[row];
-  const bool greedy = !(t > 0.f);
-  const double td = greedy ? 1.0 : static_cast<double>(t);
   rw.scale = kLog2e64 / td;
   rw.table = sh.exp2_table;
-  rw.min_p = min_p ? static_cast<double>(min_p[row]) : 0.0;
-  rw.max_key = max_in ? bin_key<T>(max_in - 1u) : 0u;
-  rw.max = Key16<T>::value(key_bits(rw.max_key));
-  const bool low_matters = max_low != 0u && !(max_in != 0u && -rw.gap(max_low) > kCntNegligible * fmax(td, 1.0));
-  const bool slow = escape != 0u || low_matters;
-  if (slow) {
-    rw.max_key = max(rw.max_key, max_all);
-    rw.max = Key16<T>::value(key_bits(rw.max_key));
-  }
+  rw.min_p = row_min;
+  rw.max_key = max_key;
+  rw.max = Key16<T>::value(key_bits(max_key));
+  const bool slow = escape != 0u || (max_low != 0u && !(-rw.gap(max_low) > kCntNegligible * fmax(td, 1.0)));
   const bool empty = rw.max_key == 0u;
 
-  // Tokens and mass of the groups whose 64 bins each start at bin `base` + 64 i, i < n, into the leader's arrays
-  // at n_before + (n - 1 - i): four bins a lane, half a warp a group, the groups spread over the cluster.
+  // Tokens and mass of the n groups of 64 bins in the counters, group i into the leader's arrays at order(i): four
+  // bins a lane, half a warp a group, the groups spread over the cluster.
   double lse = 0.0;
-  auto sum_groups = [&](int n, int n_before, auto key_of) {
+  auto sum_groups = [&](int n, auto order, auto key_of) {
     for (int i2 = rank * kCntWarps + warp; i2 * 2 < n; i2 += csize * kCntWarps) {
       const uint32_t b0 = static_cast<uint32_t>(i2) * 128 + lane * 4;
       uint32_t c[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int r = 0; r < kCntMaxCluster; ++r)
         if (r < csize) {
-          const uint2 v = *reinterpret_cast<const uint2*>(peer(hist, r) + b0 / 2);
-          c[0] += v.x & 0xffffu;
-          c[1] += v.x >> 16;
-          c[2] += v.y & 0xffffu;
-          c[3] += v.y >> 16;
+          const uint4 v = *reinterpret_cast<const uint4*>(peer(hist, r) + b0);
+          c[0] += v.x;
+          c[1] += v.y;
+          c[2] += v.z;
+          c[3] += v.w;
         }
       uint32_t num = 0;
       double m = 0.0;
@@ -303,22 +394,20 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
         uint32_t key[4];
         double w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {  // all four without branches: their chains of operations overlap
-          key[j] = key_of(b0 + j);
-          w[j] = rw.weight(key[j]);
-        }
+        for (int j = 0; j < 4; ++j) key[j] = key_of(b0 + j);
+        // the slow path's keys lie anywhere: no table
+        const bool even = !slow && key[3] <= rw.max_key && key[3] - key[0] == 3u;
+        const uint32_t binade = even ? ((key_bits(key[3]) & 0x7fffu) - Key16<T>::kBase) >> Key16<T>::kMantissa : 0u;
+        rw.mass4(key, even, sh.ratio[0][binade], rw.scale, w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t n = rw.kept(key[j], w[j]) ? c[j] : 0u;
           num += n;
-          m += n ? n * w[j] : 0.0;
+          m += n ? count_f64(n) * w[j] : 0.0;
         }
-        if (t != 1.f) {
+        if (t != 1.f) rw.mass4(key, even, sh.ratio[1][binade], kLog2e64, w);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = rw.plain(key[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lse += c[j] ? c[j] * w[j] : 0.0;
+        for (int j = 0; j < 4; ++j) lse += c[j] ? count_f64(c[j]) * w[j] : 0.0;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) {
           num += __shfl_xor_sync(0xffffffffu, num, o);
@@ -328,14 +417,14 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
       const int i = i2 * 2 + (lane >> 4);
       if ((lane & 15) == 0 && i < n) {
         CountShared* l = peer(&sh, 0);
-        l->cnt[n_before + n - 1 - i] = num;
-        l->own[n_before + n - 1 - i] = m;
+        l->cnt[order(i)] = num;
+        l->own[order(i)] = m;
       }
     }
   };
   int groups = kBins / 64;
   if (!slow) {
-    if (!empty) sum_groups(groups, 0, [](uint32_t b) { return bin_key<T>(b); });
+    if (!empty) sum_groups(groups, [](int i) { return window_order<T>(i); }, [](uint32_t b) { return bin_key<T>(b); });
   } else {
     // all 65,536 keys, kBins at a time from the top
     groups = kCntGroups;
@@ -345,16 +434,17 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
       cluster_sync();  // the window before has been read
       clear();
       __syncthreads();
-      for_each(ch0, ch1, [&](uint32_t bits) {
-        if (bits == 0x8000u) bits = 0u;
-        const uint32_t key = bits_key(bits);
-        if (key > Key16<T>::kNegInf && key <= Key16<T>::kPosInf && static_cast<int>(key) >= lo && static_cast<int>(key) < hi)
-          add(key - lo);
+      for_each(ch0, ch1, [&](uint32_t w) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = valid_key(w >> (16 * h));
+          if (key >= lo && key < hi) add(key - lo);
+        }
       });
       __syncthreads();
       cluster_sync();
       const int n = (hi - lo) / 64;
-      sum_groups(n, done, [&](uint32_t b) { return b + lo; });
+      sum_groups(n, [&](int i) { return done + n - 1 - i; }, [&](uint32_t b) { return b + lo; });
       done += n;
     }
   }
@@ -381,8 +471,22 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
     const int wper = (b - a + kCntWarps - 1) / kCntWarps;
     const int w0 = min(b, a + warp * wper), w1 = min(b, w0 + wper);
     uint32_t n = 0;
-#pragma unroll 4
-    for (int c = w0 + lane; c < w1; c += 32) n += __popc(matches(load8(c)));
+    constexpr int kAhead = 8;
+    for (int c = w0 + lane; c < w1; c += 32 * kAhead) {
+      uint4 v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int ch = c + 32 * j;
+        v[j] = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN is no candidate's pattern
+        if (ch < w1 && ch >= whole0 && ch < whole1) v[j] = __ldg(src + ch);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int ch = c + 32 * j;
+        if (ch < w1 && (ch < whole0 || ch >= whole1)) v[j] = load8(ch);
+      }
+      Key16<T>::count_equal(v, want * 0x00010001u, n);
+    }
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) sh.warp_u[0][warp] = n;
     __syncthreads();
@@ -451,15 +555,16 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
 
     // Counts of group g's values, two a lane of warp 0 in descending order, and their weights (kept ones only).
     auto load_group = [&](int g, uint32_t (&key)[2], uint32_t (&n)[2], double (&w)[2]) {
-      const uint32_t b = static_cast<uint32_t>(groups - 1 - g) * 64 + 62 - 2 * lane;  // the lower of the two bins
+      // the lower of the lane's two bins (slow: keys)
+      const uint32_t b = static_cast<uint32_t>(slow ? groups - 1 - g : window_group<T>(g)) * 64 + 62 - 2 * lane;
       n[0] = n[1] = 0;
       if (!slow) {
 #pragma unroll
         for (int r = 0; r < kCntMaxCluster; ++r)
           if (r < csize) {
-            const uint32_t v = peer(hist, r)[b / 2];
-            n[0] += v >> 16;
-            n[1] += v & 0xffffu;
+            const uint2 v = *reinterpret_cast<const uint2*>(peer(hist, r) + b);
+            n[0] += v.y;
+            n[1] += v.x;
           }
       } else {
         n[0] = sh.group_cnt[63 - 2 * lane];
@@ -482,10 +587,12 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
       if (tid < 64) sh.group_cnt[tid] = 0;
       __syncthreads();
       const uint32_t lo = static_cast<uint32_t>(groups - 1 - g) * 64;
-      for_each(0, chunks, [&](uint32_t bits) {
-        if (bits == 0x8000u) bits = 0u;
-        const uint32_t key = bits_key(bits);
-        if (key > Key16<T>::kNegInf && key <= Key16<T>::kPosInf && key - lo < 64u) atomicAdd(&sh.group_cnt[key - lo], 1u);
+      for_each(0, chunks, [&](uint32_t w) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t i = static_cast<uint32_t>(valid_key(w >> (16 * h))) - lo;
+          if (i < 64u) atomicAdd(&sh.group_cnt[i], 1u);
+        }
       });
       __syncthreads();
     };
@@ -542,8 +649,7 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
     };
 
     double kept = sh.mass[groups - 1];
-    int k = top_k ? top_k[row] : 0;
-    if (greedy || rw.min_p > 1.0) k = 1;  // the first candidate stays whatever min_p asks
+    const int k = greedy || rw.min_p > 1.0 ? 1 : row_k;  // the first candidate stays whatever min_p asks
     if (k > 0 && static_cast<uint32_t>(k) < n_all) {
       const uint32_t uk = static_cast<uint32_t>(k);
 #pragma unroll
@@ -572,13 +678,13 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
       kept = sh.cum;
       __syncthreads();
     }
-    const double p = top_p ? static_cast<double>(top_p[row]) : 1.0;
+    const double p = row_p;
     if (p < 1.0 && !greedy) {
       find_mass(fmax(p, 0.0) * kept, false);
       kept = fmin(sh.cum, kept);
       __syncthreads();
     }
-    const double uu = fmin(fmax(static_cast<double>(u[row]), 0.0), 1.0 - 0x1p-53);  // NaN: 0
+    const double uu = fmin(fmax(static_cast<double>(row_u), 0.0), 1.0 - 0x1p-53);  // NaN: 0
     find_mass(greedy ? 0.0 : uu * kept, true);
     const uint32_t key = sh.key, nth = sh.nth;
     float lp = 0.f;
@@ -596,8 +702,7 @@ __global__ void __launch_bounds__(kCntThreads, kCntThreads == 1024 ? 1 : Key16<T
       const uint32_t b = key_bin<T>(key);
       uint32_t n = 0;
       if (lane < csize) {
-        const uint32_t v = peer(hist, lane)[b / 2];
-        n = (b & 1u) ? v >> 16 : v & 0xffffu;
+        n = peer(hist, lane)[b];
       }
       const uint32_t before = warp_scan_u32(n, lane) - n;
       if (nth >= before && nth < before + n) {
@@ -622,7 +727,7 @@ template <typename T, int THREADS>
 int launch_sample_counts(const void* logits, long long ld, int rows, int V, const float* u, const float* temperature,
                          const int* top_k, const float* top_p, const float* min_p, long long* tokens, float* logprobs,
                          int csize, cudaStream_t s) {
-  constexpr int smem = static_cast<int>(2 * Key16<T>::kP * 2);
+  constexpr int smem = static_cast<int>((2 * Key16<T>::kSlots + 128) * 4);
   auto kern = sample_counts_kernel<T, THREADS>;
   cudaError_t e = smem_attr_once<sample_counts_kernel<T, THREADS>>(smem);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -646,32 +751,26 @@ template <typename T>
 int sample_counts(const void* logits, long long ld, int rows, int V, const float* u, const float* temperature,
                   const int* top_k, const float* top_p, const float* min_p, long long* tokens, float* logprobs,
                   cudaStream_t s) {
-  // a slice holds its chunks of 8 and may start 7 elements before the row
-  auto slice = [&](int c) { return ((V + 14) / 8 + c - 1) / c * 8; };
-  int csize = 1;
-  while (csize < kCntMaxCluster && slice(csize) > kCntMaxSlice) csize *= 2;
-  if (slice(csize) > kCntMaxSlice) return -2;
-  if (static_cast<long long>(rows) * csize > 0x7fffffffll) return -3;
   const long long sms = device_sm_count();
-  // few rows: spread each over more SMs, in blocks of 1024 threads, while its slices stay long enough to count
-  const bool wide = rows * static_cast<long long>(csize) <= sms;
-  const long long room = wide ? sms : sms * Key16<T>::kBlocksPerSm;
-  while (csize < kCntMaxCluster && static_cast<long long>(rows) * csize * 2 <= room && slice(csize) > 4096) csize *= 2;
-  if (wide)
+  int csize = 1;
+  // few rows: spread each over more SMs while its slices stay long enough to count
+  while (csize < kCntMaxCluster && static_cast<long long>(rows) * csize * 2 <= sms && V / csize > 4096) csize *= 2;
+  if (static_cast<long long>(rows) * csize > 0x7fffffffll) return -3;
+  if (Key16<T>::kOneRow || static_cast<long long>(rows) * csize <= sms)
     return launch_sample_counts<T, 1024>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
-  return launch_sample_counts<T, 256>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
+  return launch_sample_counts<T, 512>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
 }
 }  // namespace
 }  // namespace accerl
 
 // One token per row of logits [rows, V] (half: 0 bf16, 1 fp16; row stride ld) from u [rows]. top_k, top_p and
-// min_p may be null (off). -2: V above what a cluster can count.
+// min_p may be null (off).
 extern "C" int accerl_sample_counts(const void* logits, long long ld, int half, int rows, int V, const float* u,
                                     const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                                     long long* tokens, float* logprobs, cudaStream_t s) {
   using namespace accerl;
   if (rows <= 0) return 0;
-  if (V <= 0) return -1;
+  if (V <= 0 || V > 0x7ffffff0) return -1;
   if (half) return sample_counts<__half>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, s);
   return sample_counts<__nv_bfloat16>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, s);
 }
