@@ -353,11 +353,11 @@ def _quantize(x: torch.Tensor, pre: int, w, eps: float, out: Optional[Int8Rows])
     if x.is_cuda:
         k = x.shape[-1] // 2 if pre == 2 else x.shape[-1]
         if out is None:
-            q, scale = native().quantize_rows(x, pre, w, eps, None, None)
+            q, scale = native().quantize_rows(x, pre, w, eps, None, None, status_tensor(x.device))
             return Int8Rows(q, scale, k)
         if out.k != k:
             raise ValueError(f"out does not hold rows of {k}")
-        native().quantize_rows(x, pre, w, eps, out.q, out.scale)
+        native().quantize_rows(x, pre, w, eps, out.q, out.scale, status_tensor(x.device))
         return out
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"x must be [rows, features], got {tuple(x.shape)}")

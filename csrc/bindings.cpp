@@ -126,7 +126,7 @@ int accerl_sample_counts(const void* logits, long long ld, int half, int rows, i
                          const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                          long long* tokens, float* logprobs, cudaStream_t s);
 int accerl_quantize_rows(const void* x, long long ldx, int half, int pre, const void* w, float eps, void* q,
-                         float* scale, long long rows, int K, cudaStream_t s);
+                         float* scale, long long rows, int K, int* status, cudaStream_t s);
 int accerl_gemm_int8(const void* qx, const float* sx, const void* qw, const float* sw, int M, int N, int K,
                      const void* bias, const void* residual, long long ldr, int in_type, void* out, long long ldo,
                      int out_type, int w_early, int* status, cudaStream_t stream);
@@ -813,7 +813,7 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
 // q [rows, K rounded up to 16] and scale [rows], allocated when not given.
 std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w,
                                                  double eps, const c10::optional<at::Tensor>& q_out,
-                                                 const c10::optional<at::Tensor>& scale_out) {
+                                                 const c10::optional<at::Tensor>& scale_out, const at::Tensor& status) {
   const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be [rows, features], got ", x.sizes());
   const bool half = x.scalar_type() == at::kHalf;
@@ -847,7 +847,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pr
   }
   check(accerl_quantize_rows(x.data_ptr(), rows <= 1 ? 0 : x.stride(0), half, static_cast<int>(pre), opt_ptr(w),
                              static_cast<float>(eps), q.data_ptr(), scale.data_ptr<float>(), rows, static_cast<int>(K),
-                             cur_stream()),
+                             status.data_ptr<int>(), cur_stream()),
         "quantize_rows");
   return {q, scale};
 }
@@ -924,7 +924,7 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& qw, const at::Tens
   TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "inner dimensions differ (", x.sizes(), " vs ", K, ")");
   TORCH_CHECK_VALUE(x.device() == qw.device(), "every tensor must be on the weight's device ", qw.device(),
                     ", got one on ", x.device());
-  auto [qx, sx] = quantize_rows(x, 0, c10::nullopt, 0.0, c10::nullopt, c10::nullopt);
+  auto [qx, sx] = quantize_rows(x, 0, c10::nullopt, 0.0, c10::nullopt, c10::nullopt, status);
   if (g_last_rc != 0) return qx;  // reported by the caller
   return gemm_int8(qx, sx, qw, sw, K, bias, residual, out, out_dtype.has_value() ? out_dtype : x.scalar_type(), status,
                    true);

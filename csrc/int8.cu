@@ -10,7 +10,9 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -31,7 +33,10 @@ struct Half16;  // 16-bit float formats: unpacking of pairs and the bit pattern 
 template <>
 struct Half16<__nv_bfloat16> {
   static constexpr uint32_t kInf = 0x7f80u;
-  static ACCERL_DEVINL float2 unpack(uint32_t v) { return unpack_bf16x2(v); }
+  // one operation an element; the conversion intrinsic's code takes two for the upper half
+  static ACCERL_DEVINL float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
   static ACCERL_DEVINL float one(uint32_t bits) { return __uint_as_float(bits << 16); }
 };
 template <>
@@ -41,27 +46,23 @@ struct Half16<__half> {
   static ACCERL_DEVINL float one(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
 };
 
-// Scale of a row and the factors that turn its elements into whole numbers. `amax` is the largest
-// magnitude as a 16-bit pattern, whose order is that of the magnitudes, with infinities and NaN on top:
-// a row that holds one gets scale NaN (its outputs are NaN) and zeros.
+// A row's largest magnitude is kept as its 16-bit pattern `amax`, whose order is that of the magnitudes, with
+// infinities and NaN on top: a row that holds one gets scale NaN (its outputs are NaN) and zeros.
+template <typename T>
+ACCERL_DEVINL float row_scale(uint32_t amax) {
+  return amax >= Half16<T>::kInf ? __uint_as_float(0x7fffffffu) : __fdiv_rn(Half16<T>::one(amax), 127.f);
+}
+
+// The factors that turn a row's elements into whole numbers.
 struct RowQuant {
-  float scale, m127, a, inv;
+  float m127, a, inv;
 };
 template <typename T>
 ACCERL_DEVINL RowQuant row_quant(uint32_t amax) {
-  RowQuant o{0.f, 0.f, 0.f, 0.f};
-  if (amax >= Half16<T>::kInf) {
-    o.scale = __uint_as_float(0x7fffffffu);
-  } else if (amax != 0u) {
-    const float a = Half16<T>::one(amax);
-    // a power of two keeps 1 / a, 127 x and the remainder below inside the normal range
-    const float f = a < 0x1p-100f ? 0x1p100f : (a > 0x1p100f ? 0x1p-100f : 1.f);
-    o.scale = __fdiv_rn(a, 127.f);
-    o.a = a * f;
-    o.m127 = 127.f * f;
-    o.inv = __frcp_rn(o.a);
-  }
-  return o;
+  const float a = Half16<T>::one(amax);
+  // a power of two keeps 1 / a, 127 x and the remainder below inside the normal range
+  const float f = a < 0x1p-100f ? 0x1p100f : (a > 0x1p100f ? 0x1p-100f : 1.f);
+  return RowQuant{127.f * f, a * f, amax == 0u ? 0.f : __frcp_rn(a * f)};
 }
 
 // round_half_even(127 x / a), decided exactly without a division per element. x and a have at most 11
@@ -76,132 +77,299 @@ ACCERL_DEVINL uint32_t quant_bits(float x, const RowQuant& s) {
   const float e = __fmaf_rn(-p, s.a, n);
   return __float_as_uint(__fadd_rn(__fmaf_rn(e, s.inv, p), 0x1.8p23f));
 }
+// The same for bf16, whose 8 significant bits leave more room, with two operations instead of five: x r + 384 lies in
+// [257, 511], so the first rounds the quotient to a multiple of 2^-15, within 2^-16 of it. r's rounding moves the
+// quotient by at most 127 2^-24 < 2^-16: a tie is put back onto its border. Any other quotient is at least
+// 0.5 / (127 255) > 2^-16 + 2^-25 from a border and stays on its side. The second rounds to the nearest whole
+// number, ties to even (384 is even); the low byte is the number + 128. (Checked over all significands and
+// exponents in exact arithmetic.) For 2^-100 <= a <= 2^100; r is the quotient 127 / a by an approximate reciprocal
+// corrected by its exact remainder, which saves every thread of a row the division's code.
+ACCERL_DEVINL bool bf16_plain(uint32_t amax) { return amax >= 0x0d80u && amax <= 0x7180u; }
+ACCERL_DEVINL float bf16_ratio(uint32_t amax) {
+  const float a = __uint_as_float(amax << 16);
+  float i;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(i) : "f"(a));
+  const float q = __fmul_rn(127.f, i);
+  return __fmaf_rn(__fmaf_rn(-q, a, 127.f), i, q);
+}
+ACCERL_DEVINL uint32_t quant_bits_bf16(float x, float r) { return __float_as_uint(__fadd_rn(__fmaf_rn(x, r, 384.f), 0x1.8p23f)); }
 ACCERL_DEVINL uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// silu(g) u with the activation rounded to bf16, as swiglu_h gives it, without its division, which kept this
-// kernel at the instruction limit: the quotient g / (1 + e^-g) from an approximate reciprocal, corrected by its
-// exact remainder (Markstein, 1990). Gates beyond 80, where remainder or reciprocal could leave the normal
-// range, take swiglu_h itself.
-ACCERL_DEVINL float swiglu_row(float g, float u) {
-  if (!(fabsf(g) < 80.f)) return swiglu_h(g, u);
-  const float d = 1.f + __expf(-g);
-  const float r = __fdividef(1.f, d);
+// silu(g) for |g| < 80 before its rounding to bf16, as swiglu_h gives it but without the division, which kept this
+// kernel at the instruction limit: the quotient g / (1 + e^-g) from an approximate reciprocal, corrected by its exact
+// remainder (Markstein, 1990). The flushing forms differ from __expf's only where e^-g vanishes against 1.
+ACCERL_DEVINL float silu_small(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(g, -1.4426950408889634f)));
+  const float d = 1.f + e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
   const float q = __fmul_rn(g, r);
-  return bf16_round(__fmaf_rn(__fmaf_rn(-q, d, g), r, q)) * u;
+  return __fmaf_rn(__fmaf_rn(-q, d, g), r, q);
 }
 
-// Reduction over the `tpr` threads of a row (a power of two, 32..blockDim); `red`, one slot per warp, is used
-// by one reduction of the kernel only.
+// Reduction over the 2^lg threads of a row (32..blockDim); `red`, one slot per warp, is used by one reduction of the
+// kernel only.
 template <typename V, typename F>
-ACCERL_DEVINL V row_reduce(V v, int tpr, V* red, F f) {
+ACCERL_DEVINL V row_reduce(V v, int lg, V* red, F f) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (tpr > 32) {
+  if (lg > 5) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    const int w0 = (threadIdx.x / tpr) * (tpr >> 5);
-    v = red[w0];
-    for (int w = 1; w < (tpr >> 5); ++w) v = f(v, red[w0 + w]);
+    const int warps = 1 << (lg - 5);
+    v = red[((threadIdx.x >> lg) << (lg - 5)) + (threadIdx.x & (warps - 1))];
+    for (int o = 1; o < warps; o <<= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   }
   return v;
 }
 
 ACCERL_DEVINL uint32_t amax_pair(uint32_t m) { return max(m & 0xffffu, m >> 16); }
 
-// One row per `tpr` threads, 8 elements a thread and chunk, the row held in registers between the maximum
-// and the rounding so that it is read once. PRE turns the input row into the row to round: RMSNorm
-// (x [rows, K], weight w) or SwiGLU (x = gate | up, [rows, 2K]), with the roundings of the framework's
-// own kernels (both give rows in T).
-template <typename T, int PRE, int NC>
-__global__ void __launch_bounds__(512) quantize_rows_kernel(const T* __restrict__ x, long long ldx,
-                                                            const T* __restrict__ w, float eps,
-                                                            int8_t* __restrict__ q, float* __restrict__ scale,
-                                                            long long rows, int K, int Kp, int tpr) {
-  pdl_launch_dependents();  // the product may set itself up; it waits for this grid's end before it reads
-  __shared__ uint32_t red_u[16];
-  __shared__ float red_f[16];
-  const int in_row = threadIdx.x % tpr;
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
-  const bool live = row < rows;
-  const T* xr = x + (live ? row : 0) * ldx;
-  // every load of the row is issued up front; chunks behind its end read its first one and are zeroed
-  uint4 v[NC], up[PRE == kPreSwiglu ? NC : 1];
+// The pieces of a row that a thread holds, NC chunks of 8 elements 2^lg threads apart (packed pairs).
+// All chunks but the last lie inside the row (kWhole: NC is no rounded-up count).
+template <int NC>
+struct RowPart {
+  static constexpr bool kWhole = NC <= 5;
+  static ACCERL_DEVINL bool inside(int j, int c, int end) { return (kWhole && j < NC - 1) || c < end; }
+  uint4 v[NC];
+  ACCERL_DEVINL uint32_t* words(int j) { return reinterpret_cast<uint32_t*>(&v[j]); }
+  // gate -> silu(gate) up
+  ACCERL_DEVINL void swiglu(int j, uint4 up) {
+    const uint32_t uw[4] = {up.x, up.y, up.z, up.w};
+    uint32_t* g = words(j);
+    uint32_t m2 = 0;
 #pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    const int c = (j * tpr + in_row) * 8;
-    v[j] = *reinterpret_cast<const uint4*>(xr + (c < K ? c : 0));
-    if constexpr (PRE == kPreSwiglu) up[j] = *reinterpret_cast<const uint4*>(xr + K + (c < K ? c : 0));
-  }
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    if ((j * tpr + in_row) * 8 >= K) {
-      v[j] = make_uint4(0, 0, 0, 0);
-    } else if constexpr (PRE == kPreSwiglu) {
-      uint32_t* g = reinterpret_cast<uint32_t*>(&v[j]);
-      const uint32_t uw[4] = {up[j].x, up[j].y, up[j].z, up[j].w};
+    for (int i = 0; i < 4; ++i) m2 = __vmaxu2(m2, g[i] & 0x7fff7fffu);
+    if (amax_pair(m2) < 0x42a0u) {  // every |gate| < 80
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 fg = unpack_bf16x2(g[i]), fu = unpack_bf16x2(uw[i]);
-        g[i] = pack_bf16x2(swiglu_row(fg.x, fu.x), swiglu_row(fg.y, fu.y));
+        const float2 fg = Half16<__nv_bfloat16>::unpack(g[i]), fu = Half16<__nv_bfloat16>::unpack(uw[i]);
+        const float2 a = Half16<__nv_bfloat16>::unpack(pack_bf16x2(silu_small(fg.x), silu_small(fg.y)));
+        g[i] = pack_bf16x2(a.x * fu.x, a.y * fu.y);
+      }
+    } else {
+      for (int i = 0; i < 4; ++i) {
+        const float2 fg = Half16<__nv_bfloat16>::unpack(g[i]), fu = Half16<__nv_bfloat16>::unpack(uw[i]);
+        g[i] = pack_bf16x2(swiglu_h(fg.x, fu.x), swiglu_h(fg.y, fu.y));
       }
     }
   }
-  if constexpr (PRE == kPreRmsNorm) {
+  ACCERL_DEVINL float sum_squares() {
     float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const uint32_t* p = reinterpret_cast<const uint32_t*>(&v[j]);
+    for (int j = 0; j < NC; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack_bf16x2(p[i]);
-        ss += f.x * f.x + f.y * f.y;
+        const float2 f = Half16<__nv_bfloat16>::unpack(words(j)[i]);
+        ss = __fmaf_rn(f.y, f.y, __fmaf_rn(f.x, f.x, ss));
       }
-    }
-    ss = row_reduce(ss, tpr, red_f, [](float a, float b) { return a + b; });
-    const float r = rsqrtf(ss / static_cast<float>(K) + eps);
+    return ss;
+  }
+  // x -> bf16(bf16(x r) w), the roundings of the framework's norm
+  ACCERL_DEVINL void normalise(const __nv_bfloat16* __restrict__ w, float r, int in_row, int lg, int K) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int c = (j * tpr + in_row) * 8;
-      if (c >= K) continue;
+      const int c = ((j << lg) + in_row) * 8;
+      if (!inside(j, c, K)) continue;
       const uint4 wv = *reinterpret_cast<const uint4*>(w + c);
       const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
-      uint32_t* p = reinterpret_cast<uint32_t*>(&v[j]);
+      uint32_t* p = words(j);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack_bf16x2(p[i]), g = unpack_bf16x2(ww[i]);
-        const float2 n = unpack_bf16x2(pack_bf16x2(f.x * r, f.y * r));
+        const float2 f = Half16<__nv_bfloat16>::unpack(p[i]), g = Half16<__nv_bfloat16>::unpack(ww[i]);
+        const float2 n = Half16<__nv_bfloat16>::unpack(pack_bf16x2(f.x * r, f.y * r));
         p[i] = pack_bf16x2(n.x * g.x, n.y * g.y);
       }
     }
   }
-  uint32_t m2 = 0;
+  ACCERL_DEVINL uint32_t amax() {
+    uint32_t m2 = 0;
 #pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(&v[j]);
+    for (int j = 0; j < NC; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m2 = __vmaxu2(m2, p[i] & 0x7fff7fffu);
+      for (int i = 0; i < 4; ++i) m2 = __vmaxu2(m2, words(j)[i] & 0x7fff7fffu);
+    return amax_pair(m2);
   }
-  const uint32_t amax = row_reduce(amax_pair(m2), tpr, red_u, [](uint32_t a, uint32_t b) { return max(a, b); });
-  const RowQuant s = row_quant<T>(amax);
-  if (!live) return;
-  if (in_row == 0) scale[row] = s.scale;
-  const bool finite = amax < Half16<T>::kInf;
-  int8_t* qr = q + row * Kp;
+  // round and store; the columns K..Kp are written as zeros
+  template <typename T>
+  ACCERL_DEVINL void store(int8_t* qr, uint32_t amax, int in_row, int lg, int Kp) {
+    if (std::is_same<T, __nv_bfloat16>::value && bf16_plain(amax)) {
+      const float r = bf16_ratio(amax);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int c = ((j << lg) + in_row) * 8;
+        if (!inside(j, c, Kp)) continue;
+        uint32_t b[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = Half16<T>::unpack(words(j)[i]);
+          b[2 * i] = quant_bits_bf16(f.x, r);
+          b[2 * i + 1] = quant_bits_bf16(f.y, r);
+        }
+        *reinterpret_cast<uint2*>(qr + c) =
+            make_uint2(pack4(b[0], b[1], b[2], b[3]) ^ 0x80808080u, pack4(b[4], b[5], b[6], b[7]) ^ 0x80808080u);
+      }
+      return;
+    }
+    const bool finite = amax < Half16<T>::kInf;
+    const RowQuant s = row_quant<T>(amax);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = ((j << lg) + in_row) * 8;
+      if (!inside(j, c, Kp)) continue;
+      uint32_t b[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Half16<T>::unpack(words(j)[i]);
+        b[2 * i] = quant_bits(f.x, s);
+        b[2 * i + 1] = quant_bits(f.y, s);
+      }
+      const uint2 o = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
+      *reinterpret_cast<uint2*>(qr + c) = finite ? o : make_uint2(0, 0);
+    }
+  }
+};
+
+// One row per 2^lg threads, held in registers between the maximum and the rounding so that it is read once. PRE
+// turns the input row into the row to round: RMSNorm (x [rows, K], weight w) or SwiGLU (x = gate | up, [rows, 2K]),
+// with the roundings of the framework's own kernels (both give rows in T). For few rows: one wave of blocks.
+template <typename T, int PRE, int NC>
+__global__ void __launch_bounds__(512) quantize_rows_kernel(const T* __restrict__ x, long long ldx,
+                                                            const T* __restrict__ w, float eps,
+                                                            int8_t* __restrict__ q, float* __restrict__ scale,
+                                                            long long rows, int K, int Kp, int lg) {
+  pdl_launch_dependents();  // the product may set itself up; it waits for this grid's end before it reads
+  __shared__ uint32_t red_u[16];
+  __shared__ float red_f[16];
+  const int in_row = threadIdx.x & ((1 << lg) - 1);
+  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> lg) + (threadIdx.x >> lg);
+  const bool live = row < rows;
+  const T* xr = x + (live ? row : 0) * ldx;
+  // every load of the row is issued up front; chunks behind its end read its first one and are zeroed
+  RowPart<NC> part;
+  uint4 up[PRE == kPreSwiglu ? NC : 1];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
-    const int c = (j * tpr + in_row) * 8;
-    if (c >= Kp) continue;  // the columns K..Kp are written as zeros
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(&v[j]);
-    uint32_t b[8];
+    const int c = ((j << lg) + in_row) * 8, at = part.inside(j, c, K) ? c : 0;
+    part.v[j] = *reinterpret_cast<const uint4*>(xr + at);
+    if constexpr (PRE == kPreSwiglu) up[j] = *reinterpret_cast<const uint4*>(xr + K + at);
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Half16<T>::unpack(p[i]);
-      b[2 * i] = finite ? quant_bits(f.x, s) : 0u;
-      b[2 * i + 1] = finite ? quant_bits(f.y, s) : 0u;
+  for (int j = 0; j < NC; ++j) {
+    if (!part.inside(j, ((j << lg) + in_row) * 8, K)) part.v[j] = make_uint4(0, 0, 0, 0);
+    else if constexpr (PRE == kPreSwiglu) part.swiglu(j, up[j]);
+  }
+  if constexpr (PRE == kPreRmsNorm) {
+    const float ss = row_reduce(part.sum_squares(), lg, red_f, [](float a, float b) { return a + b; });
+    part.normalise(w, rsqrtf(ss / static_cast<float>(K) + eps), in_row, lg, K);
+  }
+  const uint32_t amax = row_reduce(part.amax(), lg, red_u, [](uint32_t a, uint32_t b) { return max(a, b); });
+  if (!live) return;
+  if (in_row == 0) scale[row] = row_scale<T>(amax);
+  part.template store<T>(q + row * Kp, amax, in_row, lg, Kp);
+}
+
+ACCERL_DEVINL void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The same for many rows (launched for SwiGLU): persistent blocks of 256 threads take 256 >> lg rows at a time out of
+// a ring of shared memory that bulk copies keep full, so that memory never waits for a row's reduction. Bound by
+// instructions more than by memory: [8192, 2 x 8960] takes 78 us of which its bytes need 56.
+constexpr int kBulkThreads = 256;
+constexpr int kBulkMaxStages = 4;
+constexpr int kBulkSmem = 74 * 1024;  // three blocks an SM
+template <typename T, int PRE, int NC>
+__global__ void __launch_bounds__(kBulkThreads) quantize_rows_bulk_kernel(const T* __restrict__ x, long long ldx,
+                                                                          const T* __restrict__ w, float eps,
+                                                                          int8_t* __restrict__ q,
+                                                                          float* __restrict__ scale, long long rows,
+                                                                          int K, int Kp, int lg, int stages,
+                                                                          int* status) {
+  extern __shared__ uint4 ring[];
+  __shared__ uint64_t full[kBulkMaxStages];
+  __shared__ uint32_t red_u[2][8];
+  __shared__ float red_f[2][8];
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = kBulkThreads >> lg;  // rows per stage
+  const int in_row = threadIdx.x & ((1 << lg) - 1), slot = threadIdx.x >> lg;
+  const uint32_t row_bytes = static_cast<uint32_t>(K) * (PRE == kPreSwiglu ? 4u : 2u);
+  const long long batches = (rows + per - 1) / per;
+  uint8_t* base = reinterpret_cast<uint8_t*>(ring);
+  auto load = [&](long long batch, int s) {  // one thread
+    const int n = static_cast<int>(min(static_cast<long long>(per), rows - batch * per));
+    mbar_arrive_expect_tx(&full[s], n * row_bytes);
+    for (int i = 0; i < n; ++i)
+      bulk_load(base + (s * per + i) * row_bytes, x + (batch * per + i) * ldx, row_bytes, &full[s]);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+    for (int s = 0; s < stages; ++s) {
+      const long long b = blockIdx.x + static_cast<long long>(s) * gridDim.x;
+      if (b < batches) load(b, s);
     }
-    *reinterpret_cast<uint2*>(qr + c) = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
+  }
+  __syncthreads();
+  int s = 0, buf = 0;
+  uint32_t phase = 0;
+  for (long long b = blockIdx.x; b < batches; b += gridDim.x) {
+    const bool ok = mbar_wait(&full[s], phase, status, kStatusTimeoutProducer);
+    const long long row = b * per + slot;
+    const bool live = row < rows;
+    const uint8_t* src = base + (s * per + slot) * row_bytes;
+    RowPart<NC> part;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = ((j << lg) + in_row) * 8;
+      if (live && part.inside(j, c, K)) {
+        part.v[j] = *reinterpret_cast<const uint4*>(src + c * 2);
+        if constexpr (PRE == kPreSwiglu) part.swiglu(j, *reinterpret_cast<const uint4*>(src + (K + c) * 2));
+      } else {
+        part.v[j] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    const int w0 = slot << (lg - 5);
+    if constexpr (PRE == kPreRmsNorm) {
+      float ss = part.sum_squares();
+      ss = warp_sum(ss);
+      if (lg > 5) {
+        if (lane == 0) red_f[buf][warp] = ss;
+        __syncthreads();
+        ss = red_f[buf][w0 + (lane & ((1 << (lg - 5)) - 1))];
+        for (int o = 1; o < (1 << (lg - 5)); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      }
+      part.normalise(w, rsqrtf(ss / static_cast<float>(K) + eps), in_row, lg, K);
+    }
+    uint32_t amax = __reduce_max_sync(0xffffffffu, part.amax());
+    if (lane == 0) red_u[buf][warp] = amax;
+    // everyone has read the stage (and the wait ran out for all or for nobody)
+    if (!__syncthreads_and(ok)) {
+      // no copy stays in flight into a finished block
+      if (threadIdx.x == 0)
+        for (int k = 0; k < stages; ++k)
+          if (b + static_cast<long long>(k) * gridDim.x < batches)
+            mbar_wait(&full[(s + k) % stages], phase ^ (s + k >= stages ? 1u : 0u), nullptr, 0, 20000000ull);
+      return;
+    }
+    const long long next = b + static_cast<long long>(stages) * gridDim.x;
+    if (threadIdx.x == 0 && next < batches) load(next, s);
+    amax = __reduce_max_sync(0xffffffffu, red_u[buf][w0 + (lane & ((1 << (lg - 5)) - 1))]);
+    if (live) {
+      if (in_row == 0) scale[row] = row_scale<T>(amax);
+      part.template store<T>(q + row * Kp, amax, in_row, lg, Kp);
+    }
+    buf ^= 1;
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1u;
+    }
   }
 }
 
@@ -217,9 +385,9 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const T* __restr
   const unsigned short* xr = reinterpret_cast<const unsigned short*>(x) + row * ldx;
   uint32_t m = 0;
   for (int c = threadIdx.x; c < K; c += blockDim.x) m = max(m, xr[c] & 0x7fffu);
-  const uint32_t amax = row_reduce(m, blockDim.x, red_u, [](uint32_t a, uint32_t b) { return max(a, b); });
+  const uint32_t amax = row_reduce(m, 8, red_u, [](uint32_t a, uint32_t b) { return max(a, b); });
   const RowQuant s = row_quant<T>(amax);
-  if (threadIdx.x == 0) scale[row] = s.scale;
+  if (threadIdx.x == 0) scale[row] = row_scale<T>(amax);
   const bool finite = amax < Half16<T>::kInf;
   for (int c = threadIdx.x; c < Kp; c += blockDim.x)
     q[row * Kp + c] = static_cast<int8_t>(
@@ -272,19 +440,12 @@ struct Int8Params {
   int* status;
 };
 
-ACCERL_DEVINL int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+ACCERL_DEVINL void st_cluster_s32(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-ACCERL_DEVINL int4 ld_cluster_s32x4(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
+// the two halves of cluster_sync
+ACCERL_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+ACCERL_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 ACCERL_DEVINL uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -334,11 +495,12 @@ ACCERL_DEVINL void finish4(const Int8Params& p, long long t, int n, int4 acc, fl
 
 // Few tokens: one tile of 128 output channels x bt tokens per cluster of CTAs. The weight rows are the MMA's
 // 128 rows, so a decode batch of few tokens wastes no tensor rows and streams the weight once. The CTAs of a
-// cluster split K (there are only N / 128 tiles to spread over 148 SMs): each leaves its integer partial in its
-// shared memory, and each sums and finishes its share of the tokens over the cluster. Integer sums have no
-// order, so the split changes no bit.
+// cluster split K (there are only N / 128 tiles to spread over 148 SMs): each sends its integer partial of a token to
+// the CTA that finishes that token (every CTA a share of them), straight from TMEM into that one's shared memory.
+// Integer sums have no order, so the split changes no bit. The two cluster barriers are split into arrival and wait:
+// the first (everybody has started) hides behind the products, the second is the only wait for the peers.
 //   warp 0: TMA producer into a ring of stages;  warp 1: TMEM and MMA issue;  warps 2-5: accumulator to
-//   shared memory;  then all warps: a token row each, four neighbouring channels a lane (VEC: 16-byte rows) or
+//   shared memory;  then all warps: a token row each, four neighbouring channels a lane (VEC: aligned rows) or
 //   every 32nd channel.
 template <int OUT, bool VEC>
 __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __grid_constant__ CUtensorMap tmW,
@@ -383,7 +545,11 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (splits > 1) cluster_arrive();
   const uint32_t tbase = tmem_slot;
+  // the tokens this CTA finishes, and where the partials of all of the cluster's CTAs for them arrive
+  const int share = p.bt / splits;
+  int* parts = reinterpret_cast<int*>(smem + (splits > 1 ? p.stages * stage_bytes : 0));
 
   if (warp == 0) {
     if (lane == 0) {
@@ -424,28 +590,43 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
       if (ok) umma_commit(&done);
     }
   } else {
+    ok = mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue);
+    tc_fence_after();
+  }
+  __syncwarp();
+  if (splits > 1) cluster_wait();
+  if (warp >= 2 && ok) {  // a timed-out wait leaves what it finds there (the status word is set)
     const int quarter = warp & 3;  // TMEM lanes this warp may read
-    if (mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue)) {
-      tc_fence_after();
-      const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16);
-      // every MMA of this CTA has read its stages: their memory takes the accumulator, [token][channel]
-      int* part = reinterpret_cast<int*>(smem) + quarter * 32 + lane;
+    const uint32_t t_row = tbase + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int ch = quarter * 32 + lane;
 #pragma unroll 1
-      for (int c0 = 0; c0 < min(p.bt, p.M - t0); c0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(t_row + c0, v);
-        tmem_wait_ld();
+    for (int c0 = 0; c0 < min(p.bt, p.M - t0); c0 += 16) {
+      uint32_t v[16];
+      tmem_ld16(t_row + c0, v);
+      tmem_wait_ld();
+      if (splits == 1) {
+        // every MMA of this CTA has read its stages: their memory takes the accumulator, [token][channel]
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[(c0 + i) * kI8Rows] = static_cast<int>(v[i]);
+        for (int i = 0; i < 16; ++i) parts[(c0 + i) * kI8Rows + ch] = static_cast<int>(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {  // [sender][token of the share][channel] at the token's owner
+          const int c = c0 + i, owner = c / share;
+          st_cluster_s32(map_shared_rank(parts + (split * share + (c - owner * share)) * kI8Rows + ch, owner),
+                         static_cast<int>(v[i]));
+        }
       }
     }
-    tc_fence_before();
   }
-  __syncthreads();
-  if (splits > 1) cluster_sync();
+  if (warp >= 2) tc_fence_before();
+  __syncwarp();
+  if (splits > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
 
-  // this CTA's share of the tokens; a timed-out wait leaves what it finds there (the status word is set)
-  const int share = (p.bt + splits - 1) / splits;
   const int c_lo = split * share, c_hi = min(min(p.bt, p.M - t0), c_lo + share);
   constexpr int kWarps = kI8Threads / 32;
   if constexpr (VEC) {
@@ -458,10 +639,10 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
                         load_as_float(p.bias, n + 2, p.in_type), load_as_float(p.bias, n + 3, p.in_type));
 #pragma unroll 2
       for (int c = c_lo + warp; c < c_hi; c += kWarps) {
-        const uint32_t off = (c * kI8Rows + lane * 4) * 4;
-        int4 acc = *reinterpret_cast<const int4*>(smem + off);
+        const int4* src = reinterpret_cast<const int4*>(parts + (c - c_lo) * kI8Rows) + lane;
+        int4 acc = *src;
         for (int r = 1; r < splits; ++r) {
-          const int4 o = ld_cluster_s32x4(map_shared_rank(smem, (split + r) % splits) + off);
+          const int4 o = src[r * share * (kI8Rows / 4)];
           acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
         }
         finish4<OUT>(p, t0 + c, n, acc, __ldg(p.sx + t0 + c), sw, b);
@@ -482,9 +663,9 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
       for (int i = 0; i < 4; ++i) {
         const int n = n0 + i * 32 + lane;
         if (n >= p.N) continue;
-        const uint32_t off = (c * kI8Rows + i * 32 + lane) * 4;
-        int acc = *reinterpret_cast<const int*>(smem + off);
-        for (int r = 1; r < splits; ++r) acc += ld_cluster_s32(map_shared_rank(smem, (split + r) % splits) + off);
+        const int* src = parts + (c - c_lo) * kI8Rows + i * 32 + lane;
+        int acc = *src;
+        for (int r = 1; r < splits; ++r) acc += src[r * share * kI8Rows];
         float y = __fmaf_rn(static_cast<float>(acc), sx * sw[i], b[i]);
         if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
         store_from_float(p.out, t * p.ldo + n, OUT, y);
@@ -492,7 +673,6 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
     }
   }
   __syncthreads();
-  if (splits > 1) cluster_sync();  // nobody leaves while its partial may still be read
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tbase, cols);
@@ -726,12 +906,10 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
         if constexpr (TMA_OUT) {
           if (p.residual && row_ok) add_residual32(f, p, row, col0);
           // 16-bit results: two buffers of 32 rows x 64 bytes; fp32: one of 32 x 128
-          uint8_t* buf = wbuf + (OUT == kOutF32 ? 0 : (chunk & 1) * (kI8EpiBytes / 2));
+          constexpr int kBufs = OUT == kOutF32 ? 1 : 2;
+          uint8_t* buf = wbuf + (chunk % kBufs) * (kI8EpiBytes / kBufs);
           ++chunk;
-          if (lane == 0) {  // the store issued from this buffer has read it
-            if constexpr (OUT == kOutF32) bulk_wait_read<0>();
-            else bulk_wait_read<1>();
-          }
+          if (lane == 0) bulk_wait_read<kBufs - 1>();  // the store issued from this buffer has read it
           __syncwarp();
           if constexpr (OUT == kOutF32) {
 #pragma unroll
@@ -765,12 +943,20 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
           const int n = col0 + lane;
           if (n < p.N) {
             const int rows = min(32, p.M - y0);
-#pragma unroll 8
-            for (int r = 0; r < rows; ++r) {
-              float y = *reinterpret_cast<const float*>(wbuf + swz128(r, lane >> 2) + (lane & 3) * 4);
-              const long long at = y0 + r;
-              if (p.residual) y += load_as_float(p.residual, at * p.ldr + n, p.in_type);
-              store_from_float(p.out, at * p.ldo + n, OUT, y);
+            for (int r0 = 0; r0 < rows; r0 += 8) {
+              float y[8];  // the residual of 8 rows is loaded before any of their results is stored
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                y[i] = p.residual && r0 + i < rows
+                           ? load_as_float(p.residual, static_cast<long long>(y0 + r0 + i) * p.ldr + n, p.in_type)
+                           : 0.f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i;
+                if (r < rows)
+                  store_from_float(p.out, static_cast<long long>(y0 + r) * p.ldo + n, OUT,
+                                   y[i] + *reinterpret_cast<const float*>(wbuf + swz128(r, lane >> 2) + (lane & 3) * 4));
+              }
             }
           }
         }
@@ -888,13 +1074,56 @@ int launch_stream(const CUtensorMap& mw, const CUtensorMap& mx, const Int8Params
   return static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_stream_kernel<OUT, VEC>, mw, mx, p));
 }
 
+// Which kernel runs a product: bt = 0 the persistent pairs, else the streaming kernel with bt tokens per tile and
+// `splits` CTAs per tile. The candidate with the least estimated cost wins. The estimate has a fixed part, a part per
+// 128 elements of K and one per token of the tile, times the share of an SM that a CTA gets; its constants are fitted
+// to the times of all candidates over M 1..4096 and eleven (K, N) from (300, 700) to (12288, 4096) so that the choice
+// is right (they are no times): the chosen candidate took 4 % longer than the best on average.
+struct Int8Plan {
+  int bt, splits;
+};
+Int8Plan plan_int8(int M, int N, int K, int sms) {
+  const int kbs = (K + kI8BK - 1) / kI8BK;
+  const double pair_tiles = static_cast<double>((M + kI8Tile - 1) / kI8Tile) * ((N + kI8Tile - 1) / kI8Tile);
+  const double waves = std::ceil(pair_tiles / (sms / 2));
+  double best = 14.3 + waves * kbs * 0.37 + (waves - 1) * 0.9;
+  Int8Plan plan{0, 1};
+  for (int bt = 16; bt <= 128 && (bt == 16 || bt < 2 * M); bt *= 2) {
+    const double tiles = static_cast<double>((M + bt - 1) / bt) * ((N + kI8Rows - 1) / kI8Rows);
+    for (int sp = 1; sp <= 8 && sp <= kbs; sp *= 2) {
+      const double ctas = tiles * sp;
+      if (sp > 1 && ctas > 4 * sms) break;
+      const double t = 6.3 + (sp > 1 ? 0.8 : 0.0) +
+                       (ctas > sms ? 2.1 * ctas / sms : 1.0) *
+                           (((kbs + sp - 1) / sp) * (0.155 + 0.00085 * bt) + 0.023 * bt);
+      if (t < best) {
+        best = t;
+        plan = Int8Plan{bt, sp};
+      }
+    }
+  }
+  return plan;
+}
+
+template <typename T, int PRE, int NC>
+int launch_quantize_bulk(const T* x, long long ldx, const T* w, float eps, int8_t* q, float* scale, long long rows,
+                         int K, int Kp, int lg, int stages, int smem, int* status, cudaStream_t s) {
+  const cudaError_t e = smem_attr_once<quantize_rows_bulk_kernel<T, PRE, NC>>(kBulkSmem);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const long long batches = (rows + (kBulkThreads >> lg) - 1) / (kBulkThreads >> lg);
+  const int resident = device_sm_count() * std::min(4, (224 * 1024) / (smem + 2048));
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(batches, resident));
+  quantize_rows_bulk_kernel<T, PRE, NC><<<grid, kBulkThreads, smem, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, lg, stages, status);
+  return static_cast<int>(cudaGetLastError());
+}
+
 template <typename T, int PRE>
 int launch_quantize(const T* x, long long ldx, const T* w, float eps, int8_t* q, float* scale, long long rows, int K,
-                    int Kp, cudaStream_t s) {
+                    int Kp, int* status, cudaStream_t s) {
   const bool vec = K % 8 == 0 && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(w) & 15) == 0;
   const int chunks = (Kp + 7) / 8;
-  if (!vec || chunks > 4 * 1024) {
+  if (!vec || chunks > 8 * 512) {
     if constexpr (PRE == kPreNone) {
       quantize_rows_any_kernel<T><<<static_cast<unsigned>(rows), 256, 0, s>>>(x, ldx, q, scale, K, Kp);
       return static_cast<int>(cudaGetLastError());
@@ -902,13 +1131,37 @@ int launch_quantize(const T* x, long long ldx, const T* w, float eps, int8_t* q,
       return -2;
     }
   }
-  // the fewest threads a row that hold it in 4 chunks each (SwiGLU: of both halves), 512 at most
-  int tpr = 32;
-  while (tpr < 512 && chunks > 4 * tpr) tpr *= 2;
-  const int block = std::max(tpr, 128);
-  const int nc = (chunks + tpr - 1) / tpr;
-  const unsigned grid = static_cast<unsigned>((rows + block / tpr - 1) / (block / tpr));
-  auto launch = [&](auto kern) { kern<<<grid, block, 0, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, tpr); };
+  // the fewest threads a row that hold it in 4 chunks each, 256 at most
+  int lg = 5;
+  while (lg < 8 && chunks > (4 << lg)) ++lg;
+  int nc = (chunks + (1 << lg) - 1) >> lg;
+  if constexpr (PRE == kPreSwiglu) {
+    // The ring pays where an SM sees many rows: SwiGLU of 8960 columns took 78 us against 91 at 8192 rows, 37 against
+    // 33 at 2048. Plain rows and RMSNorm were never faster from it (8192 x 8960: 42 us either way; 16384 x 4096
+    // RMSNorm: 60 against 49).
+    const int per = kBulkThreads >> lg;
+    const int stage = per * K * 4;
+    const int stages = std::min(kBulkMaxStages, kBulkSmem / stage);
+    if (rows > 24ll * per * device_sm_count() && nc <= 8 && stages >= 2) {
+      auto launch = [&](auto n) {
+        return launch_quantize_bulk<T, PRE, decltype(n)::value>(x, ldx, w, eps, q, scale, rows, K, Kp, lg, stages,
+                                                                stages * stage, status, s);
+      };
+      if (nc <= 1) return launch(std::integral_constant<int, 1>());
+      if (nc <= 2) return launch(std::integral_constant<int, 2>());
+      if (nc <= 3) return launch(std::integral_constant<int, 3>());
+      if (nc <= 4) return launch(std::integral_constant<int, 4>());
+      if (nc <= 5) return launch(std::integral_constant<int, 5>());
+      return launch(std::integral_constant<int, 8>());
+    }
+  }
+  if (nc > 4) {
+    lg = 9;
+    nc = (chunks + 511) / 512;
+  }
+  const int block = std::max(1 << lg, 128);
+  const unsigned grid = static_cast<unsigned>((rows + (block >> lg) - 1) / (block >> lg));
+  auto launch = [&](auto kern) { kern<<<grid, block, 0, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, lg); };
   if (nc <= 1) launch(quantize_rows_kernel<T, PRE, 1>);
   else if (nc <= 2) launch(quantize_rows_kernel<T, PRE, 2>);
   else if (nc <= 3) launch(quantize_rows_kernel<T, PRE, 3>);
@@ -924,7 +1177,7 @@ int launch_quantize(const T* x, long long ldx, const T* w, float eps, int8_t* q,
 // [rows, Kp] with Kp = K rounded up to 16 (zeros behind K) and scale [rows]. -2: a norm or SwiGLU row
 // whose size, stride or alignment does not fit 16-byte accesses.
 extern "C" int accerl_quantize_rows(const void* x, long long ldx, int half, int pre, const void* w, float eps, void* q,
-                                    float* scale, long long rows, int K, cudaStream_t s) {
+                                    float* scale, long long rows, int K, int* status, cudaStream_t s) {
   using namespace accerl;
   if (rows <= 0) return 0;
   if (K <= 0 || rows > 0x7fffffffll) return -1;
@@ -933,13 +1186,13 @@ extern "C" int accerl_quantize_rows(const void* x, long long ldx, int half, int 
   if (half) {
     if (pre != kPreNone) return -3;
     return launch_quantize<__half, kPreNone>(reinterpret_cast<const __half*>(x), ldx, nullptr, eps, qp, scale, rows, K,
-                                             Kp, s);
+                                             Kp, status, s);
   }
   const auto* xb = reinterpret_cast<const __nv_bfloat16*>(x);
   const auto* wb = reinterpret_cast<const __nv_bfloat16*>(w);
-  if (pre == kPreRmsNorm) return launch_quantize<__nv_bfloat16, kPreRmsNorm>(xb, ldx, wb, eps, qp, scale, rows, K, Kp, s);
-  if (pre == kPreSwiglu) return launch_quantize<__nv_bfloat16, kPreSwiglu>(xb, ldx, nullptr, eps, qp, scale, rows, K, Kp, s);
-  return launch_quantize<__nv_bfloat16, kPreNone>(xb, ldx, nullptr, eps, qp, scale, rows, K, Kp, s);
+  if (pre == kPreRmsNorm) return launch_quantize<__nv_bfloat16, kPreRmsNorm>(xb, ldx, wb, eps, qp, scale, rows, K, Kp, status, s);
+  if (pre == kPreSwiglu) return launch_quantize<__nv_bfloat16, kPreSwiglu>(xb, ldx, nullptr, eps, qp, scale, rows, K, Kp, status, s);
+  return launch_quantize<__nv_bfloat16, kPreNone>(xb, ldx, nullptr, eps, qp, scale, rows, K, Kp, status, s);
 }
 
 // out [M, N] (out_type) = sx sw (qx qw^T) (+ bias [N]) (+ residual [M, N]), bias and residual of in_type
@@ -968,16 +1221,17 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   p.in_type = in_type;
   p.status = status;
   p.w_early = w_early;
-  p.tiles_m = (M + kI8Tile - 1) / kI8Tile;
-  p.tiles_n = (N + kI8Tile - 1) / kI8Tile;
-  p.group_m = 8;
-  if (M > 256) {
-    CUtensorMap mx, mw, mo;
+  const Int8Plan plan = plan_int8(M, N, K, device_sm_count());
+  CUtensorMap mx, mw, mo;
+  if (plan.bt == 0) {
+    p.tiles_m = (M + kI8Tile - 1) / kI8Tile;
+    p.tiles_n = (N + kI8Tile - 1) / kI8Tile;
+    p.group_m = 8;
+    if (static_cast<long long>(p.tiles_m) * p.tiles_n > 0x3fffffff) return -4;
     if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), 128)) return -7;
     if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), 128)) return -8;
     const int rs = in_type == kOutF32 ? 4 : 2;
     const bool res_ok = !residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * rs) % 16 == 0);
-    if (static_cast<long long>(p.tiles_m) * p.tiles_n > 0x3fffffff) return -4;
     if (res_ok && make_out_map(&mo, p)) {
       if (out_type == kOutBf16) return launch_pair<kOutBf16, true>(mx, mw, mo, p, stream);
       if (out_type == kOutF16) return launch_pair<kOutF16, true>(mx, mw, mo, p, stream);
@@ -988,26 +1242,29 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
     if (out_type == kOutF16) return launch_pair<kOutF16, false>(mx, mw, mo, p, stream);
     return launch_pair<kOutF32, false>(mx, mw, mo, p, stream);
   }
-  p.bt = 16;
-  while (p.bt < M) p.bt *= 2;
+  p.bt = plan.bt;
+  const dim3 grid((N + kI8Rows - 1) / kI8Rows, (M + p.bt - 1) / p.bt, plan.splits);
+  if (grid.y > 65535) return -4;
   const int kbs = (K + kI8BK - 1) / kI8BK;
-  const int tiles = (N + kI8Rows - 1) / kI8Rows;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= device_sm_count() && splits * 2 <= kbs) splits *= 2;
   const int stage_bytes = (kI8Rows + p.bt) * kI8BK;
-  const int budget = tiles * splits > device_sm_count() ? 100 * 1024 : 200 * 1024;
-  p.stages = std::max(2, std::min({16, (kbs + splits - 1) / splits, budget / stage_bytes}));
-  // the accumulator in the end lies where the stages were
-  const int smem_bytes = std::max(p.stages * stage_bytes, p.bt * kI8Rows * 4) + 1024;
-  CUtensorMap mw, mx;
+  // the accumulator: behind the stages where peers write it, else where the stages were
+  const int acc_bytes = p.bt * kI8Rows * 4;
+  const bool alone = static_cast<long long>(grid.x) * grid.y * grid.z <= device_sm_count();  // on its SM
+  const int room = (alone ? 200 : 100) * 1024 - (plan.splits > 1 ? acc_bytes : 0);
+  p.stages = std::max(2, std::min({16, (kbs + plan.splits - 1) / plan.splits, room / stage_bytes}));
+  const int smem_bytes =
+      (plan.splits > 1 ? p.stages * stage_bytes + acc_bytes : std::max(p.stages * stage_bytes, acc_bytes)) + 1024;
   if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), kI8Rows)) return -7;
   if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), static_cast<uint32_t>(p.bt))) return -8;
-  const int es = out_type == kOutF32 ? 4 : 2, rs = in_type == kOutF32 ? 4 : 2;
-  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * es) % (4 * es) == 0 &&
+  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo % 4 == 0 &&
                    (reinterpret_cast<uintptr_t>(sw) & 15) == 0 &&
-                   (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * rs) % (4 * rs) == 0));
-  const dim3 grid(tiles, 1, splits);
-  if (out_type == kOutBf16) return vec ? launch_stream<kOutBf16, true>(mw, mx, p, grid, smem_bytes, stream) : launch_stream<kOutBf16, false>(mw, mx, p, grid, smem_bytes, stream);
-  if (out_type == kOutF16) return vec ? launch_stream<kOutF16, true>(mw, mx, p, grid, smem_bytes, stream) : launch_stream<kOutF16, false>(mw, mx, p, grid, smem_bytes, stream);
-  return vec ? launch_stream<kOutF32, true>(mw, mx, p, grid, smem_bytes, stream) : launch_stream<kOutF32, false>(mw, mx, p, grid, smem_bytes, stream);
+                   (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && ldr % 4 == 0));
+  auto launch = [&](auto type) {
+    constexpr int OUT = decltype(type)::value;
+    return vec ? launch_stream<OUT, true>(mw, mx, p, grid, smem_bytes, stream)
+               : launch_stream<OUT, false>(mw, mx, p, grid, smem_bytes, stream);
+  };
+  if (out_type == kOutBf16) return launch(std::integral_constant<int, kOutBf16>());
+  if (out_type == kOutF16) return launch(std::integral_constant<int, kOutF16>());
+  return launch(std::integral_constant<int, kOutF32>());
 }

@@ -64,7 +64,7 @@ def randn(*shape, seed=0, device="cpu", dtype=torch.bfloat16, scale=1.0):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,k", [(1, 1), (1, 1536), (3, 7), (5, 8), (7, 24), (130, 1001), (33, 8960), (2, 16400),
-                                    (2, 40000), (0, 64)])
+                                    (2, 40000), (0, 64), (6001, 256), (2500, 1544), (700, 8960), (5000, 24), (800, 32768)])
 def test_quantize_rows(device, dtype, rows, k):
     x = randn(rows, k, device=device, dtype=dtype)
     check_rows(x, ops.quantize_rows(x))
@@ -120,15 +120,20 @@ def test_quantize_rows_strides_and_out(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,k", [(1, 8), (5, 128), (64, 1536), (9, 4104), (3, 16384), (0, 64)])
+@pytest.mark.parametrize("rows,k", [(1, 8), (5, 128), (64, 1536), (9, 4104), (3, 16384), (0, 64), (6001, 200), (2500, 1544),
+                                    (701, 8960), (2, 32768), (4000, 8960), (30000, 136)])
 def test_swiglu_quantize_is_the_two_calls(device, rows, k):
     gu = randn(rows, 2 * k, device=device, scale=2.0)
+    if rows > 4:
+        gu[1] *= 40  # gates far into the saturated range
+        gu[2, 3], gu[3, 5] = float("inf"), float("nan")
     r = ops.swiglu_quantize(gu)
     check_rows(ops.swiglu(gu), r)
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,k", [(1, 8), (5, 128), (64, 1536), (9, 4104), (3, 16384), (0, 64)])
+@pytest.mark.parametrize("rows,k", [(1, 8), (5, 128), (64, 1536), (9, 4104), (3, 16384), (0, 64), (6001, 200), (2500, 1544),
+                                    (701, 8960), (2, 32768)])
 def test_rmsnorm_quantize(device, rows, k):
     """Against the norm in 64 bits: the two bf16 roundings may each fall to the other side (2^-8 of the
     value each), the maximum likewise, and the rounding to whole numbers is half a step."""
