@@ -86,6 +86,8 @@ def main():
     ap.add_argument("--warmup-seconds", type=float, default=3.0)
     ap.add_argument("--gpu-memory-utilization", type=float, default=0.8,
                     help="share of the device the engine may hold (weights + KV cache), as the reference passes to vLLM")
+    ap.add_argument("--quantization", default="none", choices=("none", "int8"),
+                    help="int8: 8-bit attention projections and dense MLPs")
     ap.add_argument("--impl", default="native", choices=("native", "reference"),
                     help="reference: the reference's own vLLM inference actor, driven by the same rollout loop")
     ap.add_argument("--json", default=None)
@@ -102,7 +104,7 @@ def main():
     args = make_args(model_path=a.model, env="synthetic", rl_algorithm="grpo", rollout_batch_size=8,
                      tw_max_episode_steps=50, tw_history_token_window=a.window, max_length=a.window,
                      infer_max_tokens=16, infer_temperature=1.0, vllm_max_num_seqs=a.max_num_seqs,
-                     vllm_max_num_batched_tokens=a.max_num_batched_tokens)
+                     vllm_max_num_batched_tokens=a.max_num_batched_tokens, infer_quantization=a.quantization)
     args.gpu_memory_utilization = a.gpu_memory_utilization
     dev = torch.device("cuda", 0)
     procs, full = [], None
@@ -141,6 +143,7 @@ def main():
         "model": a.model,
         "concurrent_trajectories": a.groups * 8,
         "max_num_seqs": a.max_num_seqs,
+        "quantization": a.quantization,
         "seconds": round(el, 2),
         "samples_produced": samples,
         "prefix_cache_hit_rate": round(st["prefix_cache_hit_rate"], 4),

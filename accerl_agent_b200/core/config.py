@@ -105,6 +105,11 @@ def build_parser() -> argparse.ArgumentParser:
     a("--device", default="auto", help="auto | cpu | cuda")
     a("--kv-cache-gb", type=float, default=None, help="KV cache size per rollout GPU (default: 60%% of free memory).")
     a("--kv-block-size", type=int, default=16)
+    a("--infer-min-p", type=float, default=0.0,
+      help="Sample only tokens whose probability is at least this share of the most likely one's (0: off).")
+    a("--infer-quantization", default="none", choices=("none", "int8"),
+      help="int8: the rollout engines run attention projections and dense MLPs in 8-bit integers with a scale per "
+           "token and output channel, quantised anew after every weight sync.")
     a("--shard-params", action="store_true",
       help="Shard parameters, gradients and optimizer state over the FSDP ranks per decoder layer "
            "(all-gathered before each layer's forward and backward, gradients reduce-scattered after "
@@ -249,6 +254,8 @@ def validate_args(args: argparse.Namespace, check_games: bool = True) -> None:
         raise ValueError("--infer-temperature must be >= 0")
     if not 0.0 < args.infer_top_p <= 1.0:
         raise ValueError("--infer-top-p must be in (0, 1]")
+    if not 0.0 <= args.infer_min_p <= 1.0:
+        raise ValueError("--infer-min-p must be in [0, 1]")
     if args.num_rollout_workers < 1:
         raise ValueError("--num-rollout-workers must be >= 1")
     if args.num_rollout_workers < args.fsdp_world_size:

@@ -20,7 +20,14 @@ and then prefill chunks of waiting ones under ``max_num_batched_tokens`` / ``max
 forward over the mixed batch (new K/V written straight into their paged slots, prefill queries over
 their cached prefix with the varlen attention kernel, decode queries with the paged decode kernel),
 applies the LM head only to rows that sample, and samples on the device (temperature, top-k,
-top-p; ``csrc/sampler.cu``), which also returns each sampled token's log-probability. Sampled ids come back to the host once per step.
+top-p; ``csrc/sampler.cu``), which also returns each sampled token's log-probability. Requests with
+``min_p`` are sampled from numbers keyed by (seed, position) with ``ops.sample_inverse_cdf``. Sampled ids
+come back to the host once per step.
+
+``quantization="int8"`` runs the attention projections and the dense MLPs in 8-bit integers
+(``ops.linear_int8``: a scale per token and per output channel): their weights are quantised on the engine's
+GPU when the first step after a weight update is launched, norms and SwiGLU write 8-bit rows directly. The
+embedding, LM head, MoE experts and the KV cache keep the engine's type.
 """
 
 from __future__ import annotations
@@ -41,7 +48,7 @@ from .. import ops
 from ..utils import nvtx
 from ..models.config import ModelConfig
 from ..models.transformer import CausalLM, ParamLayout
-from .generation import SamplingParams
+from .generation import SamplingParams, uniform_numbers
 from .kv_cache import BlockAllocator, block_hash
 
 
@@ -126,12 +133,14 @@ class GenerationEngine:
         tp_group=None,
         cmd_group=None,
         async_steps: bool = True,
+        quantization: Optional[str] = None,
     ):
         """``layout``: flat parameter layout of the engine (default: the full-model layout); pass the
         trainer's layout to make weight syncs plain range copies. ``tp_group``/``cmd_group``: process
         groups of a tensor-parallel engine (NCCL for the activations' all-reduce, gloo for the step
         commands the leader, group rank 0, broadcasts); rank r then holds the r-th shard of every
-        tensor-parallel weight and ranks > 0 run ``serve_follower``."""
+        tensor-parallel weight and ranks > 0 run ``serve_follower``. ``quantization``: None or
+        ``"int8"`` (see the module's docstring)."""
         if device.type == "cuda" and device.index is None:  # the step thread selects this exact GPU
             device = torch.device("cuda", torch.cuda.current_device())
         self.full_cfg = cfg
@@ -171,6 +180,18 @@ class GenerationEngine:
         if params is None:
             params = torch.zeros(self.layout.total_numel, dtype=dtype, device=device)
         self.model = CausalLM(cfg, self.layout, params, None)
+        if quantization not in (None, "int8"):
+            raise ValueError(f"quantization must be None or 'int8', got {quantization!r}")
+        self.quantization = quantization
+        # the 8-bit copies of the projection weights, allocated before the KV cache takes the rest
+        self._w8: Dict[str, ops.Int8Rows] = {}
+        self._w8_stale = quantization is not None
+        self._w8_event = None  # end of the last asynchronous copy into the weights
+        if quantization is not None:
+            if device.type == "cuda" and (dtype != torch.bfloat16 or cfg.hidden_size % 8 or cfg.intermediate_size % 8):
+                raise ValueError("int8 on the GPU needs bf16 and hidden and intermediate sizes that are multiples of 8")
+            self._refresh_int8()
+            self._w8_stale = True
         L, Hkv, D = cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim
         per_block = 2 * L * block_size * Hkv * D * torch.tensor([], dtype=dtype).element_size()
         if num_blocks is None:
@@ -287,6 +308,8 @@ class GenerationEngine:
             # accepted by the vLLM-shaped parameter object but not applied by this engine's sampler:
             # refuse instead of sampling without it
             raise ValueError("frequency_penalty is not supported by the native engine")
+        if not 0.0 <= getattr(sampling_params, "min_p", 0.0) <= 1.0:
+            raise ValueError(f"min_p must be in [0, 1], got {sampling_params.min_p}")
         if self._thread is None:
             self.start()
         loop = asyncio.get_running_loop()
@@ -377,7 +400,35 @@ class GenerationEngine:
         with self._step_lock:
             self._flush()
             load_hf_checkpoint(self.model, path)
+            self.weights_changed()
             self.allocator.clear_cache()
+
+    def weights_changed(self, stream=None) -> None:
+        """Note that the weights were written (on ``stream``, default the current one): the 8-bit copies
+        are made anew when the next step is launched. Called by every weight update of this class; callers
+        that write ``model.params`` themselves call it afterwards."""
+        if self.quantization is None:
+            return
+        if self.device.type == "cuda":
+            with torch.cuda.device(self.device):
+                self._w8_event = (stream or torch.cuda.current_stream(self.device)).record_event()
+        self._w8_stale = True
+
+    def _refresh_int8(self) -> None:
+        """Quantise the projection weights into their 8-bit copies, in place (captured graphs read them)."""
+        if not self._w8_stale:
+            return
+        if self._w8_event is not None:
+            torch.cuda.current_stream(self.device).wait_event(self._w8_event)
+            self._w8_event = None
+        for layer in range(self.cfg.num_hidden_layers):
+            p = f"model.layers.{layer}."
+            names = ["self_attn.qkv_proj.weight", "self_attn.o_proj.weight"]
+            if not self.cfg.layer_is_moe(layer):
+                names += ["mlp.gate_up_proj.weight", "mlp.down_proj.weight"]
+            for name in names:
+                self._w8[p + name] = ops.quantize_rows(self.model.w(p + name), out=self._w8.get(p + name))
+        self._w8_stale = False
 
     def load_flat_weights(self, src: torch.Tensor, start: int = 0, stream=None) -> None:
         """Copy a fused-layout flat weight range (from a trainer, possibly a peer GPU's memory)."""
@@ -389,6 +440,7 @@ class GenerationEngine:
                     dst.copy_(src, non_blocking=True)
             else:
                 dst.copy_(src, non_blocking=True)
+            self.weights_changed(stream)
 
     def set_weight_source(self, src_layout: ParamLayout, tensor: Optional[torch.Tensor] = None,
                           addr: Optional[int] = None) -> None:
@@ -460,6 +512,7 @@ class GenerationEngine:
             nbytes += map_bytes(descs, dst.element_size())
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
+        self.weights_changed()
         return nbytes
 
     def get_stats(self) -> Dict[str, Any]:
@@ -615,6 +668,7 @@ class GenerationEngine:
     def _launch(self, plan) -> Dict[str, Any]:
         """Launch one step (prefill chunks eagerly, single-token rows from a decode graph when all of
         them sample) and commit its optimistic bookkeeping. Returns the handle ``_complete`` reads."""
+        self._refresh_int8()
         prefill = [p for p in plan if p[2] > 1]
         decode = [p for p in plan if p[2] == 1]
         parts = []
@@ -696,18 +750,24 @@ class GenerationEngine:
             dist.all_reduce(y, group=self.tp_group)
         return y
 
-    def _row_parallel(self, a: torch.Tensor, w: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
-        """``residual + a @ w^T`` for a row-parallel weight: every rank multiplies its column slice
-        and the partial sums are all-reduced. With peer access the GEMM writes its partial into the
+    def _row_parallel(self, a, w, residual: torch.Tensor) -> torch.Tensor:
+        """``residual + a @ w^T`` for a row-parallel weight (a tensor, or ``Int8Rows``, whose rows ``a``
+        may be quantised already): every rank multiplies its column slice and the partial sums are
+        all-reduced. With peer access the GEMM writes its partial into the
         symmetric buffer and one P2P kernel sums the ranks and adds the residual; otherwise rank 0
         adds the residual in the GEMM epilogue and NCCL (gloo on CPU) all-reduces."""
         if self._tp_ar is not None:
             k = self._ar_calls
             self._ar_calls += 1
             part = self._tp_ar.slot(k, a.shape[0], w.shape[0])
-            ops.linear(a, w, out=part)
+            linear = ops.linear_int8 if isinstance(w, ops.Int8Rows) else ops.linear
+            linear(a, w, out=part)
             return self._tp_ar.reduce(k, part, residual)
-        y = ops.linear(a, w, residual=residual if self.tp_rank == 0 else None)
+        mine = residual if self.tp_rank == 0 else None
+        if isinstance(w, ops.Int8Rows):
+            y = ops.linear_int8(a, w, residual=mine, out_dtype=residual.dtype)
+        else:
+            y = ops.linear(a, w, residual=mine)
         return self._all_reduce(y)
 
     def _reduce_partial(self, y: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
@@ -727,20 +787,31 @@ class GenerationEngine:
         attention output rows. Returns the final hidden rows (before the last norm)."""
         cfg, m = self.cfg, self.model
         D, Hq, Hkv = cfg.head_dim, cfg.num_attention_heads, cfg.num_key_value_heads
+        w8 = self._w8
         self._ar_calls = 0
         for layer in range(cfg.num_hidden_layers):
             p = f"model.layers.{layer}."
-            h1, _ = ops.rmsnorm(x, m.w(p + "input_layernorm.weight"), cfg.rms_norm_eps)
             bias = m.w(p + "self_attn.qkv_proj.bias") if cfg.qkv_bias else None
-            qkv = ops.linear(h1, m.w(p + "self_attn.qkv_proj.weight"), bias=bias)
+            if w8:
+                h1 = ops.rmsnorm_quantize(x, m.w(p + "input_layernorm.weight"), cfg.rms_norm_eps)
+                qkv = ops.linear_int8(h1, w8[p + "self_attn.qkv_proj.weight"], bias=bias, out_dtype=x.dtype)
+            else:
+                h1, _ = ops.rmsnorm(x, m.w(p + "input_layernorm.weight"), cfg.rms_norm_eps)
+                qkv = ops.linear(h1, m.w(p + "self_attn.qkv_proj.weight"), bias=bias)
             kc, vc = self.k_cache[layer], self.v_cache[layer]
             qn = m.w(p + "self_attn.q_norm.weight") if cfg.qk_norm else None
             kn = m.w(p + "self_attn.k_norm.weight") if cfg.qk_norm else None
             # qk-norm, RoPE and the cache write in one kernel
             ops.qkv_rope_cache(qkv, pos_d, slots_d, kc, vc, Hq, Hkv, cfg.rope_theta, qn, kn, cfg.rms_norm_eps)
             attn = attn_fn(layer, qkv[:, : cfg.q_dim], kc, vc)
-            x = self._row_parallel(attn, m.w(p + "self_attn.o_proj.weight"), x)
-            h2, _ = ops.rmsnorm(x, m.w(p + "post_attention_layernorm.weight"), cfg.rms_norm_eps)
+            x = self._row_parallel(attn, w8[p + "self_attn.o_proj.weight"] if w8 else m.w(p + "self_attn.o_proj.weight"), x)
+            post = m.w(p + "post_attention_layernorm.weight")
+            if w8 and not cfg.layer_is_moe(layer):
+                h2 = ops.rmsnorm_quantize(x, post, cfg.rms_norm_eps)
+                gu = ops.linear_int8(h2, w8[p + "mlp.gate_up_proj.weight"], out_dtype=x.dtype)
+                x = self._row_parallel(ops.swiglu_quantize(gu), w8[p + "mlp.down_proj.weight"], x)
+                continue
+            h2, _ = ops.rmsnorm(x, post, cfg.rms_norm_eps)
             if cfg.layer_is_moe(layer):
                 from ..models.moe import moe_forward
 
@@ -756,7 +827,7 @@ class GenerationEngine:
 
     def _decode_core(self, ids_d, pos_d, slots_d, table_d, lens_d, temps_d, seeds_d, offs_d, splits: int,
                      rowslot_d=None):
-        """Forward of single-token rows (every row samples): returns (tokens, logprobs) on device.
+        """Forward of single-token rows (every row samples): returns (tokens, logprobs, logits) on device.
         Rows whose id is negative read their input token from the slot table (``rowslot_d``), and the
         sampled tokens are written back into it."""
         cfg, m = self.cfg, self.model
@@ -775,10 +846,10 @@ class GenerationEngine:
         tok, lp = ops.sample(logits, temps_d, seeds_d, offs_d)
         if rowslot_d is not None:
             self._slot_tok.index_copy_(0, rowslot_d, tok)
-        return tok, lp
+        return tok, lp, logits
 
-    def _graph_for(self, bucket: int, width: int):
-        key = (bucket, width)
+    def _graph_for(self, bucket: int, width: int, keep_logits: bool = False):
+        key = (bucket, width, keep_logits)
         g = self._graphs.get(key)
         if g is not None:
             return g
@@ -818,8 +889,11 @@ class GenerationEngine:
             self._graph_pool = torch.cuda.graph_pool_handle()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, pool=self._graph_pool):
-            out_tok, out_lp = run()
-        g = {"graph": graph, "meta": meta, "temps": temps, "offs": offs, "tok": out_tok, "lp": out_lp}
+            out_tok, out_lp, logits = run()
+        # only graphs whose steps hold min-p rows keep their logits; the others share that memory
+        g = {"graph": graph, "meta": meta, "temps": temps, "offs": offs, "tok": out_tok, "lp": out_lp,
+             "logits": logits if keep_logits else None}
+        del logits
         self._graphs[key] = g
         return g
 
@@ -859,10 +933,11 @@ class GenerationEngine:
         temps[:n] = np.fromiter((float(s.params.temperature) for s, *_ in order), dtype=np.float32, count=n)
         offs = np.zeros(bucket, dtype=np.int64)
         offs[:n] = np.fromiter((len(s.out) + s.pending for s, *_ in order), dtype=np.int64, count=n)
-        return {"kind": "graph", "B": B, "bucket": bucket, "width": width, "host": host, "temps": temps, "offs": offs}
+        return {"kind": "graph", "B": B, "bucket": bucket, "width": width, "host": host, "temps": temps, "offs": offs,
+                "min_p": _min_p_rows([s for s, *_ in order])}
 
     def _run_graph(self, meta):
-        g = self._graph_for(meta["bucket"], meta["width"])
+        g = self._graph_for(meta["bucket"], meta["width"], meta["min_p"] is not None)
         n_meta = g["meta"].numel()
         bk = meta["bucket"]
         host = np.empty(n_meta + 2 * bk, dtype=np.int64)
@@ -875,7 +950,25 @@ class GenerationEngine:
         g["temps"].copy_(d[n_meta + bk :].view(torch.float32)[:bk])
         g["graph"].replay()
         B = meta["B"]
+        if meta["min_p"] is not None:
+            self._resample(meta["min_p"], g["logits"], g["tok"], g["lp"])
+            self._slot_tok.index_copy_(0, g["meta"][5 * bk : 5 * bk + B], g["tok"][:B])
         return self._stage_results(g["tok"][:B], g["lp"][:B])
+
+    def _resample(self, rows_meta, logits: torch.Tensor, tokens: torch.Tensor, lps: torch.Tensor) -> None:
+        """Sample the rows that ask for min-p from their given numbers, over the batch's results."""
+        n = len(rows_meta["rows"])
+        host = np.empty(4 * n, dtype=np.int64)
+        host[:n] = rows_meta["rows"]
+        host[n : 2 * n] = rows_meta["top_k"]
+        host[2 * n :].view(np.float32)[:] = rows_meta["floats"].reshape(-1)
+        d = self._h2d(host)
+        rows = d[:n]
+        u, temps, top_p, min_p = d[2 * n :].view(torch.float32).view(4, n).unbind(0)
+        picked = logits if n == logits.shape[0] else logits.index_select(0, rows)
+        tok, lp = ops.sample_inverse_cdf(picked, u, temps, top_k=d[n : 2 * n].to(torch.int32), top_p=top_p, min_p=min_p)
+        tokens.index_copy_(0, rows, tok)
+        lps.index_copy_(0, rows, lp)
 
     def _execute_decode_graph(self, order):
         meta = self._graph_meta(order)
@@ -949,6 +1042,7 @@ class GenerationEngine:
         meta["offs"] = np.asarray([len(sq.out) + sq.pending for sq, *_ in sampled], np.int64)
         if any(sq.params.top_p < 1.0 or (sq.params.top_k or -1) > 0 for sq, *_ in sampled):
             meta["filter_params"] = [sq.params for sq, *_ in sampled]
+        meta["min_p"] = _min_p_rows([sq for sq, *_ in sampled])
         return meta
 
     def _execute(self, order, n_prefill: int):
@@ -1034,6 +1128,8 @@ class GenerationEngine:
                 tokens, lps = ops.sample(logits, temps_d, seeds_d, offs_d, top_k=top_k, top_p=top_p)
             else:
                 tokens, lps = ops.sample(logits, temps_d, seeds_d, offs_d)
+            if meta["min_p"] is not None:
+                self._resample(meta["min_p"], logits, tokens, lps)
             self._slot_tok.index_copy_(0, rowslot_d.index_select(0, rows_d), tokens.to(torch.long))
             return self._stage_results(tokens, lps)  # the one device->host copy of the step
 
@@ -1063,6 +1159,7 @@ class GenerationEngine:
             if kind == "stop":
                 return
             if kind == "step":
+                self._refresh_int8()
                 if payload["kind"] == "graph":
                     _, _, ev = self._run_graph(payload)
                 else:
@@ -1133,6 +1230,22 @@ class GenerationEngine:
         if len(seq.out) >= p.max_tokens or seq.length >= self.max_model_len:
             return "length"
         return None
+
+
+def _min_p_rows(seqs) -> Optional[Dict[str, Any]]:
+    """Host inputs of the rows among the sampled sequences ``seqs`` that ask for min-p (None without any):
+    row indices, top-k, and [u, temperature, top-p, min-p]."""
+    rows = [i for i, s in enumerate(seqs) if getattr(s.params, "min_p", 0.0) > 0.0]
+    if not rows:
+        return None
+    picked = [seqs[i] for i in rows]
+    u = uniform_numbers(np.asarray([s.seed for s in picked], np.int64),
+                        np.asarray([len(s.out) + s.pending for s in picked], np.int64))
+    return {"rows": np.asarray(rows, np.int64),
+            "top_k": np.asarray([max(int(s.params.top_k or 0), 0) for s in picked], np.int64),
+            "floats": np.asarray([u, [float(s.params.temperature) for s in picked],
+                                  [float(s.params.top_p) for s in picked],
+                                  [float(s.params.min_p) for s in picked]], np.float32)}
 
 
 def _decode_splits(ctas_per_split: int) -> int:

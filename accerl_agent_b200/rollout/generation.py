@@ -33,6 +33,8 @@ import uuid
 from dataclasses import dataclass, field
 from typing import Any, Dict, List, Literal, Optional
 
+import numpy as np
+
 StopReason = Literal["length", "stop", "tool_calls", "abort"]
 _TERMINAL = ("stop", "tool_calls", "length")
 
@@ -53,6 +55,8 @@ class SamplingParams:
     logprobs: Optional[int] = None
     skip_special_tokens: bool = True
     frequency_penalty: float = 0.0
+    # keep the tokens whose tempered probability is at least min_p times the largest one's (0: off)
+    min_p: float = 0.0
     seed: Optional[int] = None
     # "cumulative": a RequestOutput after every step (streaming); "final_only": only the finished
     # (or aborted) output, which saves the per-step hand-off for callers that use only the last one
@@ -62,7 +66,7 @@ class SamplingParams:
         for name, default in (
             ("temperature", 1.0), ("top_p", 1.0), ("top_k", -1), ("max_tokens", 16), ("stop", None),
             ("stop_token_ids", None), ("ignore_eos", False), ("logprobs", None), ("skip_special_tokens", True),
-            ("frequency_penalty", 0.0), ("seed", None), ("output_kind", "cumulative"),
+            ("frequency_penalty", 0.0), ("min_p", 0.0), ("seed", None), ("output_kind", "cumulative"),
         ):
             setattr(self, name, kwargs.pop(name, default))
         kwargs.pop("use_beam_search", None)
@@ -70,6 +74,17 @@ class SamplingParams:
             raise TypeError(f"Unsupported sampling parameters: {sorted(kwargs)}")
         if self.top_k is not None and self.top_k >= 10**7:
             self.top_k = -1
+
+
+def uniform_numbers(seeds: np.ndarray, positions: np.ndarray) -> np.ndarray:
+    """float32 numbers in [0, 1), a function of (seed, position) alone: the upper 24 bits of SplitMix64 (Steele,
+    Lea and Flood, 2014), started at the seed and advanced ``position + 1`` steps."""
+    with np.errstate(over="ignore"):
+        z = seeds.astype(np.uint64) + (positions.astype(np.uint64) + np.uint64(1)) * np.uint64(0x9E3779B97F4A7C15)
+        z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+        z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+        z = z ^ (z >> np.uint64(31))
+    return ((z >> np.uint64(40)).astype(np.float64) * 2.0 ** -24).astype(np.float32)
 
 
 @dataclass
@@ -267,10 +282,11 @@ class InterruptibleGenerationRunner(ResumableFrontEnd):
 
     def __init__(self, engine, temperature: float = 0.7, top_p: float = 0.9,
                  stop_sequences: Optional[List[str]] = None, collect_logprobs: bool = False,
-                 max_resubmit_retries: int = 200, sampling_params_cls=SamplingParams):
+                 max_resubmit_retries: int = 200, sampling_params_cls=SamplingParams, min_p: float = 0.0):
         super().__init__(engine, max_resubmit_retries, sampling_params_cls)
         self.temperature = temperature
         self.top_p = top_p
+        self.min_p = min_p
         self.stop_sequences = stop_sequences or ["</answer>"]
         self.collect_logprobs = collect_logprobs
 
@@ -281,6 +297,8 @@ class InterruptibleGenerationRunner(ResumableFrontEnd):
     def sampling_kwargs(self, budget: int, ctx=None) -> Dict[str, Any]:
         kw: Dict[str, Any] = {"temperature": self.temperature, "top_p": self.top_p, "max_tokens": budget,
                               "stop": self.stop_sequences}
+        if self.min_p > 0.0:
+            kw["min_p"] = self.min_p
         if self.collect_logprobs:
             kw["logprobs"] = 1
         return kw

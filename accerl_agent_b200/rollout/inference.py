@@ -61,6 +61,7 @@ def build_engine(args, device: torch.device, tokenizer=None, dtype: Optional[tor
         tokenizer=tokenizer,
         tp_group=tp_group,
         cmd_group=cmd_group,
+        quantization=None if getattr(args, "infer_quantization", "none") == "none" else args.infer_quantization,
     )
 
 
@@ -81,7 +82,7 @@ class InferenceService:
             stop = ["\n"]
         self.runner = InterruptibleGenerationRunner(
             self.engine, temperature=args.infer_temperature, top_p=args.infer_top_p, stop_sequences=stop,
-            collect_logprobs=True,
+            collect_logprobs=True, min_p=getattr(args, "infer_min_p", 0.0),
         )
         if stop is None:
             self.runner.stop_sequences = None
