@@ -11,7 +11,7 @@
 // exponential per value that occurs, and only integer atomics, so a result does not depend on their order.
 //
 // Counters for all values would not fit an SM. The kernel counts a window of the values that logits take (bf16: zero
-// and 2^-40 to 2^24; fp16: below 64, each sign) in 64 KB (168 KB). Lower values, masks of the type's lowest value
+// and 2^-40 to 2^24; fp16: below 128, each sign) in 64 KB (176 KB). Lower values, masks of the type's lowest value
 // among them, are left out where they weigh nothing; a row with any other value takes the slow path, which counts
 // all values, window by window.
 #include <cuda_fp16.h>
@@ -56,13 +56,19 @@ struct Key16<__nv_bfloat16> {
     }
     n += static_cast<uint32_t>(__low2float(sum) + __high2float(sum));
   }
+  static ACCERL_DEVINL uint32_t min2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
   // halves that are not 0 where w, whose magnitude is t - 0x8000 + kBase, is not in the window
   static ACCERL_DEVINL uint32_t outside(uint32_t w, uint32_t t) { return (t & 0xe000e000u) ^ 0x80008000u; }
+  // top bit of the halves whose magnitude lies below the window
+  static ACCERL_DEVINL uint32_t below(uint32_t t) { return ~t; }
 };
 template <>
 struct Key16<__half> {
   static constexpr uint32_t kInf = 0x7c00u, kPosInf = 0xfc00u, kNegInf = 0x03ffu;
-  static constexpr uint32_t kBase = 0u, kSlots = 21u << 10, kMantissa = 10;
+  static constexpr uint32_t kBase = 0u, kSlots = 22u << 10, kMantissa = 10;
   static constexpr bool kOneRow = true;
   static ACCERL_DEVINL float value(uint32_t bits) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
@@ -82,6 +88,11 @@ struct Key16<__half> {
     }
     n += static_cast<uint32_t>(__low2float(sum) + __high2float(sum));
   }
+  static ACCERL_DEVINL uint32_t min2(uint32_t a, uint32_t b) {
+    const __half2 m = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  static ACCERL_DEVINL uint32_t below(uint32_t t) { return ~(t - 0x00010001u); }
   static ACCERL_DEVINL uint32_t outside(uint32_t w, uint32_t t) {
     return (~(t - 0x00010001u) | ((w & 0x7fff7fffu) + (0x8000u - kSlots) * 0x00010001u)) & 0x80008000u;
   }
@@ -134,6 +145,9 @@ ACCERL_DEVINL uint32_t warp_scan_u32(uint32_t v, int lane) {
   }
   return v;
 }
+ACCERL_DEVINL void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+ACCERL_DEVINL void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 template <typename V>
 ACCERL_DEVINL V* peer(V* p, int rank) {  // the same shared variable in CTA `rank` of the cluster
   return static_cast<V*>(__cluster_map_shared_rank(p, rank));
@@ -149,9 +163,11 @@ struct CountShared {
   double warp_d[32];
   double exp2_table[64];            // 2^(j / 64)
   double ratio[2][64];              // of neighbouring values' masses by binade of the window: at T, at 1
-  uint32_t max_key, max_low, escape;          // of this CTA's slice: keys, and whether a value escapes the window
+  // of every CTA's slice: the largest key, whether a value lies below the window, whether one escapes it otherwise
+  uint32_t max_key[kCntMaxCluster], any_low[kCntMaxCluster], escape[kCntMaxCluster];
   uint32_t group_cnt[64];                     // slow path: tokens of a group's values
-  int found;                                  // a search's group
+  int found[3];                               // the searches' groups (top-k, top-p, draw)
+  double log_sum;                             // leader: log of the sum of exp(x - max)
   uint32_t key, nth;                          // its value and rank among the value's tokens
   double cum;                                 // mass up to and with that token
   int nth_here;                               // rank of the drawn token within this CTA's slice, or -1
@@ -168,11 +184,10 @@ ACCERL_DEVINL double exp2_64th(double y, const double* table) {
   const double t = y + 0x1.8p52;
   const int n = __double2loint(t);
   const double r = (y - (t - 0x1.8p52)) * (0.693147180559945309417 / 64);
-  double q = __fma_rn(r, 1.0 / 120, 1.0 / 24);
-  q = __fma_rn(q, r, 1.0 / 6);
-  q = __fma_rn(q, r, 0.5);
-  q = __fma_rn(q, r, 1.0);
-  q = __fma_rn(q, r, 1.0) * table[n & 63];
+  // (1 + r) + r^2 ((1/2 + r/6) + r^2 (1/24 + r/120)): the dependent operations are what this costs
+  const double r2 = r * r;
+  const double hi = __fma_rn(r2, __fma_rn(r, 1.0 / 120, 1.0 / 24), __fma_rn(r, 1.0 / 6, 0.5));
+  const double q = __fma_rn(r2, hi, 1.0 + r) * table[n & 63];
   const double v = __hiloint2double(__double2hiint(q) + (n >> 6) * 0x100000, __double2loint(q));
   return y < -64.0 * 1020 ? 0.0 : v;
 }
@@ -197,14 +212,19 @@ struct RowWeights {
   }
   ACCERL_DEVINL double weight(uint32_t key) const { return mass(key, scale); }
   ACCERL_DEVINL double plain(uint32_t key) const { return mass(key, kLog2e64); }  // exp(x - max)
-  // masses of four neighbouring keys, ascending; `even`: equally spaced and none above the maximum, so that
-  // each is the one above it times the ratio r
+  // masses of four neighbouring keys, ascending; `even`: equally spaced, each is the one above it times the ratio r,
+  // from the largest that is not above the row's maximum on
   ACCERL_DEVINL void mass4(const uint32_t (&key)[4], bool even, double r, double sc, double (&w)[4]) const {
     if (even) {
-      w[3] = mass(key[3], sc);
-      w[2] = w[3] * r;
-      w[1] = w[2] * r;
-      w[0] = w[1] * r;
+      // `above` of the keys lie above the maximum and hold nothing
+      const uint32_t above = key[3] > max_key ? min(key[3] - max_key, 4u) : 0u;
+      const double m0 = mass(key[3] - above, sc), r2 = r * r;
+      const double m[4] = {m0, m0 * r, m0 * r2, (m0 * r) * r2};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // key[j] is 3 - j - above steps below the first
+        const uint32_t d = 3u - j;
+        w[j] = d < above ? 0.0 : (d - above == 0u ? m[0] : d - above == 1u ? m[1] : d - above == 2u ? m[2] : m[3]);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = mass(key[j], sc);
@@ -247,31 +267,38 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  // f(word) for every two elements of the chunks [a, b). Whole chunks are loaded without a branch, several in
-  // flight a thread; the one or two at the row's ends that are not whole are one thread's.
+  // chunks [whole0, whole1) lie inside the row
   const int whole0 = head ? 1 : 0, whole1 = (head + V) / 8;
+  constexpr int kAhead = 2;
   const uint4* src = reinterpret_cast<const uint4*>(x - head);
-  auto for_each = [&](int a, int b, auto f) {
-    constexpr int kAhead = 4;
-    const int a1 = max(a, whole0), b1 = min(b, whole1);
-    auto words = [&](uint4 v) {
-      f(v.x);
-      f(v.y);
-      f(v.z);
-      f(v.w);
-    };
-    int c = a1 + tid;
-    for (; c + (kAhead - 1) * kCntThreads < b1; c += kCntThreads * kAhead) {
-      uint4 v[kAhead];
+  // this thread's kAhead chunks from c on; behind `end` NaN, which nothing counts
+  auto load_batch = [&](uint4 (&v)[kAhead], int c, int end) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j] = __ldg(src + c + j * kCntThreads);
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) words(v[j]);
+    for (int j = 0; j < kAhead; ++j) {
+      const int ch = c + j * kCntThreads;
+      v[j] = ch >= whole0 && ch < min(end, whole1) ? __ldg(src + ch) : make_uint4(~0u, ~0u, ~0u, ~0u);
     }
-    for (; c < b1; c += kCntThreads) words(__ldg(src + c));
-    if (tid == 0) {
-      if (a < whole0 && a < b) words(load8(a));
-      if (b > whole1 && whole1 >= max(a, whole0)) words(load8(whole1));
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {  // the row's ends
+      const int ch = c + j * kCntThreads;
+      if (ch < end && (ch < whole0 || ch >= whole1)) v[j] = load8(ch);
+    }
+  };
+  // f(word) for every two elements of the chunks [a, b), the next batch on its way while one is worked on; `v`
+  // holds the first
+  auto for_each = [&](uint4 (&v)[kAhead], int a, int b, auto f) {
+#pragma unroll 1
+    for (int c = a + tid; c < b; c += kAhead * kCntThreads) {
+      uint4 next[kAhead];
+      load_batch(next, c + kAhead * kCntThreads, b);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        f(v[j].x);
+        f(v[j].y);
+        f(v[j].z);
+        f(v[j].w);
+        v[j] = next[j];
+      }
     }
   };
   auto valid_key = [](uint32_t w) -> int {  // -1: -inf or NaN
@@ -282,12 +309,30 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     for (int i = tid; i < static_cast<int>((kBins + 64) / 4); i += kCntThreads) dyn[i] = make_uint4(0, 0, 0, 0);
   };
   auto add = [&](uint32_t bin) { atomicAdd(&hist[bin], 1u); };
+  // the same under a predicate, not a branch
+  const uint32_t hist_smem = smem_u32(hist);
+  auto add_unless = [&](uint32_t skip, uint32_t bin) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.eq.u32 p, %1, 0;\n"
+        "@p red.shared::cta.add.u32 [%0], 1;\n"
+        "}\n" ::"r"(hist_smem + bin * 4u),
+        "r"(skip)
+        : "memory");
+  };
 
   // the row's settings, on their way while the slice is counted
   const float t = temperature[row], row_u = u[row];
   const float row_p = top_p ? top_p[row] : 1.f, row_min = min_p ? min_p[row] : 0.f;
   const int row_k = top_k ? top_k[row] : 0;
+  // the first loads travel while the counters are cleared
+  uint4 batch[kAhead];
+  load_batch(batch, ch0 + tid, ch1);
+  __syncwarp();
+  cluster_arrive_relaxed();
   clear();
+  if (tid < 3) sh.found[tid] = kCntGroups;
   if (tid == 0) sh.nth_here = -1;
   const bool greedy = !(t > 0.f);
   const double td = greedy ? 1.0 : static_cast<double>(t);
@@ -300,83 +345,94 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
   __syncthreads();
 
   // ---- count the slice ----
-  uint32_t max2 = 0xffffffffu, max_low = 0, escape = 0;  // NaN: loses to everything
-  for_each(ch0, ch1, [&](uint32_t w) {
-    // Both halves at once, with plain 32-bit operations (the integer pipe is what bounds this loop): no sum of a
-    // half carries or borrows. With slot = magnitude - kBase, t = 0x8000 + slot, its complement for a negative value
-    // is 0x7fff - slot, and v - (0x8000 - 64 - kSlots) is the bin of either sign.
-    constexpr uint32_t kOnes = 0x00010001u, kOff = 0x8000u - 64u - S;
-    max2 = Key16<T>::max2(max2, w);
-    const uint32_t t = (w | 0x80008000u) - Key16<T>::kBase * kOnes, v = t ^ half_masks(w);
+  uint32_t max2 = 0xffffffffu, min2 = 0xffffffffu, low2 = 0;  // NaN: loses to everything
+  for_each(batch, ch0, ch1, [&](uint32_t w) {
+    // Both halves at once, with plain 32-bit operations and no branch (instructions are what bounds this loop): no sum
+    // of a half carries or borrows. With slot = magnitude - kBase, t = 0x8000 + slot, its complement for a negative
+    // value is 0x7fff - slot, and v - (0x8000 - 64 - kSlots) is the bin of either sign.
+    constexpr uint32_t kOff = 0x8000u - 64u - S;
+    const uint32_t t = (w | 0x80008000u) - Key16<T>::kBase * 0x00010001u, v = t ^ half_masks(w);
     const uint32_t out = Key16<T>::outside(w, t);
-    if (!(out & 0xffffu)) add((v & 0xffffu) - kOff);
-    if (!(out >> 16)) add((v >> 16) - kOff);
-    // zeros and finite values outside the window; infinities and NaN have the top bit of `special` (+inf shows in
-    // max2, the others are nothing)
-    const uint32_t special = (w & 0x7fff7fffu) + (0x8000u - Key16<T>::kInf) * kOnes;
-    const uint32_t odd = (out & 0xffffu && !(special & 0x8000u) ? 1u : 0u) | (out >> 16 && !(special >> 31) ? 2u : 0u);
-    if (odd) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (!(odd & (1u << h))) continue;
-        const uint32_t bits = (w >> (16 * h)) & 0xffffu, m = bits & 0x7fffu;
-        if (m == 0u) add(0u);
-        else if (m >= Key16<T>::kBase + S && bits != m) max_low = max(max_low, bits_key(bits));
-        else escape = 1u;
+    add_unless(out & 0xffffu, (v & 0xffffu) - kOff);
+    add_unless(out & 0xffff0000u, (v >> 16) - kOff);
+    max2 = Key16<T>::max2(max2, w);
+    min2 = Key16<T>::min2(min2, w);
+    low2 |= Key16<T>::below(t);
+  });
+  uint32_t escape = 0;
+  if (low2 & 0x80008000u) {  // zeros, or magnitudes below the window
+    for (int c = ch0 + tid; c < ch1; c += kCntThreads) {
+      const uint4 q = load8(c);
+      const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t mag = (qw[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
+        if (mag == 0u) add(0u);
+        else if (static_cast<int>(mag) < static_cast<int>(Key16<T>::kBase)) escape = 1u;
       }
     }
-  });
-  max2 = Key16<T>::max2(max2, max2 >> 16 | max2 << 16) & 0xffffu;
-  uint32_t max_key = (max2 & 0x7fffu) > Key16<T>::kInf ? 0u : bits_key((max2 & 0x7fffu) ? max2 : 0u);
+  }
+  // the largest and the smallest of both halves as keys (0: there is nothing but NaN)
+  auto one_key = [](uint32_t bits) -> uint32_t {
+    bits &= 0xffffu;
+    return (bits & 0x7fffu) > Key16<T>::kInf ? 0u : bits_key((bits & 0x7fffu) ? bits : 0u);
+  };
+  uint32_t max_key = one_key(Key16<T>::max2(max2, max2 >> 16));
   if (max_key <= Key16<T>::kNegInf) max_key = 0u;
-  if (max_key == Key16<T>::kPosInf) escape = 1u;
+  if (max_key >= 0x8000u + Key16<T>::kBase + S) escape = 1u;  // above the window
+  // whether anything (-inf at least) lies below the window
+  const uint32_t min_key = one_key(Key16<T>::min2(min2, min2 >> 16));
+  uint32_t any_low = min_key != 0u && min_key <= 0x7fffu - Key16<T>::kBase - S ? 1u : 0u;
   max_key = __reduce_max_sync(0xffffffffu, max_key);
-  max_low = __reduce_max_sync(0xffffffffu, max_low);
+  any_low = __reduce_max_sync(0xffffffffu, any_low);
   escape = __reduce_max_sync(0xffffffffu, escape);
   if (lane == 0) {
     sh.warp_u[0][warp] = max_key;
-    sh.warp_u[1][warp] = max_low;
+    sh.warp_u[1][warp] = any_low;
     sh.warp_u[2][warp] = escape;
   }
   __syncthreads();
+  cluster_wait_all();  // everybody has started
   if (warp == 0) {
     const bool has = lane < kCntWarps;
     max_key = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[0][lane] : 0u);
-    max_low = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[1][lane] : 0u);
+    any_low = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[1][lane] : 0u);
     escape = __reduce_max_sync(0xffffffffu, has ? sh.warp_u[2][lane] : 0u);
-    if (lane == 0) {
-      sh.max_key = max_key;
-      sh.max_low = max_low;
-      sh.escape = escape;
+    if (lane < csize) {  // to every CTA of the cluster
+      CountShared* o = peer(&sh, lane);
+      o->max_key[rank] = max_key;
+      o->any_low[rank] = any_low;
+      o->escape[rank] = escape;
     }
   }
   __syncthreads();
   cluster_sync();
 
   // ---- the row's largest value, and whether the window holds all that matters ----
-  max_key = max_low = escape = 0;
-#pragma unroll
-  for (int c = 0; c < kCntMaxCluster; ++c)
-    if (c < csize) {
-      const CountShared* o = peer(&sh, c);
-      max_key = max(max_key, o->max_key);
-      max_low = max(max_low, o->max_low);
-      escape |= o->escape;
-    }
+  max_key = any_low = escape = 0;
+  for (int c = 0; c < csize; ++c) {
+    max_key = max(max_key, sh.max_key[c]);
+    any_low |= sh.any_low[c];
+    escape |= sh.escape[c];
+  }
   RowWeights<T> rw;
   rw.scale = kLog2e64 / td;
   rw.table = sh.exp2_table;
   rw.min_p = row_min;
   rw.max_key = max_key;
   rw.max = Key16<T>::value(key_bits(max_key));
-  const bool slow = escape != 0u || (max_low != 0u && !(-rw.gap(max_low) > kCntNegligible * fmax(td, 1.0)));
+  // what lies below the window is at most its lower edge
+  const float edge = -Key16<T>::value(Key16<T>::kBase + S);
+  const bool low_matters =
+      !(static_cast<double>(rw.max) - static_cast<double>(edge) > kCntNegligible * fmax(td, 1.0));
+  const bool slow = max_key != 0u && (escape != 0u || (any_low != 0u && low_matters));
   const bool empty = rw.max_key == 0u;
 
   // Tokens and mass of the n groups of 64 bins in the counters, group i into the leader's arrays at order(i): four
   // bins a lane, half a warp a group, the groups spread over the cluster.
   double lse = 0.0;
   auto sum_groups = [&](int n, auto order, auto key_of) {
-    for (int i2 = rank * kCntWarps + warp; i2 * 2 < n; i2 += csize * kCntWarps) {
+    // neighbouring pairs of groups, which are either all populated or all empty, to different CTAs
+    for (int i2 = warp * csize + rank; i2 * 2 < n; i2 += csize * kCntWarps) {
       const uint32_t b0 = static_cast<uint32_t>(i2) * 128 + lane * 4;
       uint32_t c[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -391,23 +447,35 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       uint32_t num = 0;
       double m = 0.0;
       if (__any_sync(0xffffffffu, (c[0] | c[1] | c[2] | c[3]) != 0u)) {
+        // the leader's counters of these bins, which nobody else reads, take the whole cluster's counts
+        if (csize > 1) *reinterpret_cast<uint4*>(peer(hist, 0) + b0) = make_uint4(c[0], c[1], c[2], c[3]);
         uint32_t key[4];
         double w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) key[j] = key_of(b0 + j);
         // the slow path's keys lie anywhere: no table
-        const bool even = !slow && key[3] <= rw.max_key && key[3] - key[0] == 3u;
+        const bool even = !slow && key[3] - key[0] == 3u;
         const uint32_t binade = even ? ((key_bits(key[3]) & 0x7fffu) - Key16<T>::kBase) >> Key16<T>::kMantissa : 0u;
+        auto take = [&](const double (&at_t)[4], const double (&at_1)[4]) {
+          double mk[4], ml[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t k = rw.kept(key[j], at_t[j]) ? c[j] : 0u;
+            num += k;
+            mk[j] = k ? count_f64(k) * at_t[j] : 0.0;
+            ml[j] = c[j] ? count_f64(c[j]) * at_1[j] : 0.0;
+          }
+          m = (mk[0] + mk[1]) + (mk[2] + mk[3]);
+          lse += (ml[0] + ml[1]) + (ml[2] + ml[3]);
+        };
         rw.mass4(key, even, sh.ratio[0][binade], rw.scale, w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t n = rw.kept(key[j], w[j]) ? c[j] : 0u;
-          num += n;
-          m += n ? count_f64(n) * w[j] : 0.0;
+        if (t == 1.f) {
+          take(w, w);
+        } else {  // the two chains of operations overlap
+          double w1[4];
+          rw.mass4(key, even, sh.ratio[1][binade], kLog2e64, w1);
+          take(w, w1);
         }
-        if (t != 1.f) rw.mass4(key, even, sh.ratio[1][binade], kLog2e64, w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lse += c[j] ? count_f64(c[j]) * w[j] : 0.0;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) {
           num += __shfl_xor_sync(0xffffffffu, num, o);
@@ -434,7 +502,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       cluster_sync();  // the window before has been read
       clear();
       __syncthreads();
-      for_each(ch0, ch1, [&](uint32_t w) {
+      load_batch(batch, ch0 + tid, ch1);
+      for_each(batch, ch0, ch1, [&](uint32_t w) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int key = valid_key(w >> (16 * h));
@@ -471,17 +540,17 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     const int wper = (b - a + kCntWarps - 1) / kCntWarps;
     const int w0 = min(b, a + warp * wper), w1 = min(b, w0 + wper);
     uint32_t n = 0;
-    constexpr int kAhead = 8;
-    for (int c = w0 + lane; c < w1; c += 32 * kAhead) {
-      uint4 v[kAhead];
+    constexpr int kBatch = 8;
+    for (int c = w0 + lane; c < w1; c += 32 * kBatch) {
+      uint4 v[kBatch];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
+      for (int j = 0; j < kBatch; ++j) {
         const int ch = c + 32 * j;
         v[j] = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN is no candidate's pattern
         if (ch < w1 && ch >= whole0 && ch < whole1) v[j] = __ldg(src + ch);
       }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
+      for (int j = 0; j < kBatch; ++j) {
         const int ch = c + 32 * j;
         if (ch < w1 && (ch < whole0 || ch >= whole1)) v[j] = load8(ch);
       }
@@ -552,6 +621,13 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     }
     __syncthreads();
     const uint32_t n_all = sh.cnt[groups - 1];
+    if (warp == kCntWarps - 1) {
+      double sum = 0.0;
+      for (int i = lane; i < csize * kCntWarps; i += 32) sum += sh.lse[i];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) sh.log_sum = log(sum);
+    }
 
     // Counts of group g's values, two a lane of warp 0 in descending order, and their weights (kept ones only).
     auto load_group = [&](int g, uint32_t (&key)[2], uint32_t (&n)[2], double (&w)[2]) {
@@ -559,13 +635,9 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       const uint32_t b = static_cast<uint32_t>(slow ? groups - 1 - g : window_group<T>(g)) * 64 + 62 - 2 * lane;
       n[0] = n[1] = 0;
       if (!slow) {
-#pragma unroll
-        for (int r = 0; r < kCntMaxCluster; ++r)
-          if (r < csize) {
-            const uint2 v = *reinterpret_cast<const uint2*>(peer(hist, r) + b);
-            n[0] += v.y;
-            n[1] += v.x;
-          }
+        const uint2 v = *reinterpret_cast<const uint2*>(hist + b);
+        n[0] = v.y;
+        n[1] = v.x;
       } else {
         n[0] = sh.group_cnt[63 - 2 * lane];
         n[1] = sh.group_cnt[62 - 2 * lane];
@@ -587,7 +659,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       if (tid < 64) sh.group_cnt[tid] = 0;
       __syncthreads();
       const uint32_t lo = static_cast<uint32_t>(groups - 1 - g) * 64;
-      for_each(0, chunks, [&](uint32_t w) {
+      load_batch(batch, tid, chunks);
+      for_each(batch, 0, chunks, [&](uint32_t w) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t i = static_cast<uint32_t>(valid_key(w >> (16 * h))) - lo;
@@ -597,9 +670,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       __syncthreads();
     };
     // The first position whose cumulative mass reaches (strict: exceeds) `limit` -> sh.key, sh.nth, sh.cum.
-    auto find_mass = [&](double limit, bool strict) {
-      if (tid == 0) sh.found = kCntGroups;
-      __syncthreads();
+    auto find_mass = [&](int* found, double limit, bool strict) {
       int mine = kCntGroups, last = -1;
 #pragma unroll
       for (int j = kCntPer - 1; j >= 0; --j) {
@@ -609,16 +680,16 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
           if (strict ? m[j] > limit : m[j] >= limit) mine = g;
         }
       }
-      if (mine < kCntGroups) atomicMin(&sh.found, mine);
+      if (mine < kCntGroups) atomicMin(found, mine);
       __syncthreads();
-      if (sh.found == kCntGroups) {  // rounding at the very end: the last group that has mass
+      if (*found == kCntGroups) {  // rounding at the very end: the last group that has mass
         __syncthreads();
-        if (tid == 0) sh.found = -1;
+        if (tid == 0) *found = -1;
         __syncthreads();
-        if (last >= 0) atomicMax(&sh.found, last);
+        if (last >= 0) atomicMax(found, last);
         __syncthreads();
       }
-      const int g = sh.found;
+      const int g = *found;
       recount(g);
       if (warp == 0) {
         uint32_t key[2], n[2];
@@ -655,10 +726,10 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
 #pragma unroll
       for (int j = 0; j < kCntPer; ++j) {
         const int g = tid * kCntPer + j;
-        if (g < groups && c[j] >= uk && (g == 0 || (j ? c[j - 1] : cb) < uk)) sh.found = g;
+        if (g < groups && c[j] >= uk && (g == 0 || (j ? c[j - 1] : cb) < uk)) sh.found[0] = g;
       }
       __syncthreads();
-      const int g = sh.found;
+      const int g = sh.found[0];
       recount(g);
       if (warp == 0) {
         uint32_t key[2], n[2];
@@ -680,30 +751,23 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     }
     const double p = row_p;
     if (p < 1.0 && !greedy) {
-      find_mass(fmax(p, 0.0) * kept, false);
+      find_mass(&sh.found[1], fmax(p, 0.0) * kept, false);
       kept = fmin(sh.cum, kept);
       __syncthreads();
     }
     const double uu = fmin(fmax(static_cast<double>(row_u), 0.0), 1.0 - 0x1p-53);  // NaN: 0
-    find_mass(greedy ? 0.0 : uu * kept, true);
+    find_mass(&sh.found[2], greedy ? 0.0 : uu * kept, true);
     const uint32_t key = sh.key, nth = sh.nth;
-    float lp = 0.f;
-    if (warp == 0 || slow) {
-      double s = 0.0;
-      for (int i = lane; i < csize * kCntWarps; i += 32) s += sh.lse[i];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      lp = static_cast<float>((key == rw.max_key ? 0.0 : rw.gap(key)) - log(s));
-    }
+    const float lp = static_cast<float>((key == rw.max_key ? 0.0 : rw.gap(key)) - sh.log_sum);
     if (slow) {
       write_token(0, chunks, key, nth, lp);
     } else if (warp == 0) {
       // the CTA whose slice holds the nth of them: lane r asks CTA r
       const uint32_t b = key_bin<T>(key);
-      uint32_t n = 0;
-      if (lane < csize) {
-        n = peer(hist, lane)[b];
-      }
+      uint32_t n = lane < csize ? peer(hist, lane)[b] : 0u;
+      // the leader's holds everybody's
+      const uint32_t others = __reduce_add_sync(0xffffffffu, lane ? n : 0u);
+      if (lane == 0 && csize > 1) n -= others;
       const uint32_t before = warp_scan_u32(n, lane) - n;
       if (nth >= before && nth < before + n) {
         CountShared* o = peer(&sh, lane);
@@ -751,14 +815,15 @@ template <typename T>
 int sample_counts(const void* logits, long long ld, int rows, int V, const float* u, const float* temperature,
                   const int* top_k, const float* top_p, const float* min_p, long long* tokens, float* logprobs,
                   cudaStream_t s) {
-  const long long sms = device_sm_count();
+  // Few rows: spread each over more SMs while its slices stay long enough to count. Measured on V = 151936 (bf16, us
+  // by cluster size 1, 2, 4, 8): 1 row 38, 27, 20, 16; 64 rows 52, 35, 30, 46; 150 rows 65, 57, 62, 98; 256 rows 72,
+  // 74, 93, 156. Blocks of 1024 threads, one an SM, are what fp16's counters leave room for (bf16: 79 for 256 rows).
+  constexpr int threads = Key16<T>::kOneRow ? 1024 : 512;
+  const long long resident = static_cast<long long>(device_sm_count()) * (1024 / threads) * 21 / 20;
   int csize = 1;
-  // few rows: spread each over more SMs while its slices stay long enough to count
-  while (csize < kCntMaxCluster && static_cast<long long>(rows) * csize * 2 <= sms && V / csize > 4096) csize *= 2;
+  while (csize < kCntMaxCluster && static_cast<long long>(rows) * csize * 2 <= resident && V / csize > 4096) csize *= 2;
   if (static_cast<long long>(rows) * csize > 0x7fffffffll) return -3;
-  if (Key16<T>::kOneRow || static_cast<long long>(rows) * csize <= sms)
-    return launch_sample_counts<T, 1024>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
-  return launch_sample_counts<T, 512>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
+  return launch_sample_counts<T, threads>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
 }
 }  // namespace
 }  // namespace accerl
