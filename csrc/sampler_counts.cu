@@ -750,17 +750,23 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       __syncthreads();
     }
     const double p = row_p;
-    if (p < 1.0 && !greedy) {
-      find_mass(&sh.found[1], fmax(p, 0.0) * kept, false);
-      kept = fmin(sh.cum, kept);
-      __syncthreads();
-    }
     const double uu = fmin(fmax(static_cast<double>(row_u), 0.0), 1.0 - 0x1p-53);  // NaN: 0
-    find_mass(&sh.found[2], greedy ? 0.0 : uu * kept, true);
+    // the cut by top-p, then the draw (a loop: one copy of the search's code)
+#pragma unroll 1
+    for (int stage = p < 1.0 && !greedy ? 1 : 2; stage <= 2; ++stage) {
+      find_mass(&sh.found[stage], stage == 1 ? fmax(p, 0.0) * kept : (greedy ? 0.0 : uu * kept), stage == 2);
+      if (stage == 1) {
+        kept = fmin(sh.cum, kept);
+        __syncthreads();
+      }
+    }
     const uint32_t key = sh.key, nth = sh.nth;
     const float lp = static_cast<float>((key == rw.max_key ? 0.0 : rw.gap(key)) - sh.log_sum);
     if (slow) {
-      write_token(0, chunks, key, nth, lp);
+      if (tid == 0) {  // the leader goes through the whole row
+        sh.nth_here = static_cast<int>(nth);
+        sh.logprob = lp;
+      }
     } else if (warp == 0) {
       // the CTA whose slice holds the nth of them: lane r asks CTA r
       const uint32_t b = key_bin<T>(key);
@@ -783,7 +789,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
   }
   __syncthreads();
   cluster_sync();  // the draw is known, and nobody reads another's memory any more
-  if (sh.nth_here >= 0) write_token(ch0, ch1, sh.key, static_cast<uint32_t>(sh.nth_here), sh.logprob);
+  if (sh.nth_here >= 0)
+    write_token(slow ? 0 : ch0, slow ? chunks : ch1, sh.key, static_cast<uint32_t>(sh.nth_here), sh.logprob);
 }
 
 namespace {
