@@ -21,6 +21,11 @@ namespace accerl {
 // ------------------------------------------------------------------------------------------------
 // rows to 8 bits
 // ------------------------------------------------------------------------------------------------
+// Arrival at a named barrier without waiting.
+ACCERL_DEVINL void named_bar_arrive(uint32_t id, uint32_t nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
 // Programmatic dependent launch: a product launched behind its quantising kernel starts while that one still
 // runs, sets itself up and waits here for the whole grid before it and its memory.
 ACCERL_DEVINL void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -419,6 +424,7 @@ ACCERL_DEVINL void umma_s8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint
 
 constexpr int kI8BK = 128;         // elements (= bytes) of K per stage: one 128-byte swizzled row
 constexpr int kI8Rows = 128;       // weight rows per tile
+constexpr int kI8MaxTokens = 128;  // per tile of the streaming kernel
 constexpr int kI8Threads = 192;
 
 enum OutType : int { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2 };
@@ -445,6 +451,7 @@ ACCERL_DEVINL void st_cluster_s32(uint32_t addr, int v) {
 }
 // the two halves of cluster_sync
 ACCERL_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+ACCERL_DEVINL void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 ACCERL_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 ACCERL_DEVINL uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -510,6 +517,7 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[16], empty[16], done;
   __shared__ uint32_t tmem_slot;
+  __shared__ float sx_s[kI8MaxTokens];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * kI8Rows, t0 = blockIdx.y * p.bt;
   const int split = blockIdx.z, splits = gridDim.z;
@@ -521,35 +529,58 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   while (cols < static_cast<uint32_t>(p.bt)) cols <<= 1;
   bool ok = true;
   int issued = 0;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  // warp 0 goes on to its loads as soon as the barriers stand; the others meet behind the TMEM allocation
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < p.stages; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(&done, 1);
+      fence_mbar_init();
     }
-    mbar_init(&done, 1);
-    fence_mbar_init();
-    // the first weight tiles start at once, behind a quantising kernel even before the tokens are there
-    // (p.w_early: nothing that kernel writes is part of the weight)
-    if (!p.w_early) pdl_wait();
-    for (; issued < min(p.stages, kbs); ++issued) {
-      mbar_arrive_expect_tx(&full[issued], stage_bytes);
-      tma_load_2d(smem + issued * stage_bytes, &tmW, &full[issued], (kb_first + issued) * kI8BK, n0);
+    __syncwarp();
+    named_bar_arrive(1, kI8Threads);
+    if (lane == 0) {
+      // behind a quantising kernel the first weight tiles start even before the tokens are there (p.w_early: nothing
+      // that kernel writes is part of the weight)
+      if (!p.w_early) pdl_wait();
+      for (; issued < min(p.stages, kbs); ++issued) {
+        mbar_arrive_expect_tx(&full[issued], stage_bytes);
+        tma_load_2d(smem + issued * stage_bytes, &tmW, &full[issued], (kb_first + issued) * kI8BK, n0);
+        if (!p.w_early)
+          tma_load_2d(smem + issued * stage_bytes + kI8Rows * kI8BK, &tmX, &full[issued], (kb_first + issued) * kI8BK, t0);
+      }
+      if (p.w_early) {
+        pdl_wait();
+        for (int s = 0; s < issued; ++s)
+          tma_load_2d(smem + s * stage_bytes + kI8Rows * kI8BK, &tmX, &full[s], (kb_first + s) * kI8BK, t0);
+      }
     }
-    pdl_wait();
-    for (int s = 0; s < issued; ++s)
-      tma_load_2d(smem + s * stage_bytes + kI8Rows * kI8BK, &tmX, &full[s], (kb_first + s) * kI8BK, t0);
+    __syncwarp();
+  } else {
+    if (warp == 1) tmem_alloc(&tmem_slot, cols);
+    tc_fence_before();
+    named_bar_sync(1, kI8Threads);
+    tc_fence_after();
   }
-  __syncwarp();
-  if (warp == 1) tmem_alloc(&tmem_slot, cols);
   pdl_wait();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (splits > 1) cluster_arrive();
-  const uint32_t tbase = tmem_slot;
+  if (splits > 1) cluster_arrive_relaxed();  // nothing to publish yet: only that this CTA has started
+  const uint32_t tbase = warp == 0 ? 0u : tmem_slot;
   // the tokens this CTA finishes, and where the partials of all of the cluster's CTAs for them arrive
-  const int share = p.bt / splits;
+  const int share = p.bt / splits, share_lg = 31 - __clz(share);  // powers of two
   int* parts = reinterpret_cast<int*>(smem + (splits > 1 ? p.stages * stage_bytes : 0));
+  // the lane's channel scales and bias, loaded long before they are used
+  float4 sw = make_float4(0.f, 0.f, 0.f, 0.f), b = sw;
+  if constexpr (VEC) {
+    const int n = n0 + lane * 4;
+    if (n < p.N) {
+      sw = *reinterpret_cast<const float4*>(p.sw + n);
+      if (p.bias)
+        b = make_float4(load_as_float(p.bias, n, p.in_type), load_as_float(p.bias, n + 1, p.in_type),
+                        load_as_float(p.bias, n + 2, p.in_type), load_as_float(p.bias, n + 3, p.in_type));
+    }
+  }
 
   if (warp == 0) {
     if (lane == 0) {
@@ -590,6 +621,7 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
       if (ok) umma_commit(&done);
     }
   } else {
+    for (int i = threadIdx.x - 64; i < p.bt; i += 128) sx_s[i] = t0 + i < p.M ? p.sx[t0 + i] : 0.f;
     ok = mbar_wait(&done, 0, p.status, kStatusTimeoutEpilogue);
     tc_fence_after();
   }
@@ -611,8 +643,8 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {  // [sender][token of the share][channel] at the token's owner
-          const int c = c0 + i, owner = c / share;
-          st_cluster_s32(map_shared_rank(parts + (split * share + (c - owner * share)) * kI8Rows + ch, owner),
+          const int c = c0 + i, owner = c >> share_lg;
+          st_cluster_s32(map_shared_rank(parts + (split * share + (c & (share - 1))) * kI8Rows + ch, owner),
                          static_cast<int>(v[i]));
         }
       }
@@ -632,12 +664,7 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   if constexpr (VEC) {
     const int n = n0 + lane * 4;
     if (n < p.N) {  // N is a multiple of 4
-      const float4 sw = *reinterpret_cast<const float4*>(p.sw + n);
-      float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p.bias)
-        b = make_float4(load_as_float(p.bias, n, p.in_type), load_as_float(p.bias, n + 1, p.in_type),
-                        load_as_float(p.bias, n + 2, p.in_type), load_as_float(p.bias, n + 3, p.in_type));
-#pragma unroll 2
+#pragma unroll 4
       for (int c = c_lo + warp; c < c_hi; c += kWarps) {
         const int4* src = reinterpret_cast<const int4*>(parts + (c - c_lo) * kI8Rows) + lane;
         int4 acc = *src;
@@ -645,20 +672,20 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
           const int4 o = src[r * share * (kI8Rows / 4)];
           acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
         }
-        finish4<OUT>(p, t0 + c, n, acc, __ldg(p.sx + t0 + c), sw, b);
+        finish4<OUT>(p, t0 + c, n, acc, sx_s[c], sw, b);
       }
     }
   } else {
-    float sw[4], b[4];
+    float sc[4], bi[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = n0 + i * 32 + lane;
-      sw[i] = n < p.N ? p.sw[n] : 0.f;
-      b[i] = (n < p.N && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
+      sc[i] = n < p.N ? p.sw[n] : 0.f;
+      bi[i] = (n < p.N && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
     }
     for (int c = c_lo + warp; c < c_hi; c += kWarps) {
       const long long t = t0 + c;
-      const float sx = __ldg(p.sx + t);
+      const float sx = sx_s[c];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int n = n0 + i * 32 + lane;
@@ -666,7 +693,7 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
         const int* src = parts + (c - c_lo) * kI8Rows + i * 32 + lane;
         int acc = *src;
         for (int r = 1; r < splits; ++r) acc += src[r * share * kI8Rows];
-        float y = __fmaf_rn(static_cast<float>(acc), sx * sw[i], b[i]);
+        float y = __fmaf_rn(static_cast<float>(acc), sx * sc[i], bi[i]);
         if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
         store_from_float(p.out, t * p.ldo + n, OUT, y);
       }
@@ -1006,10 +1033,9 @@ bool make_int8_map(CUtensorMap* out, const void* ptr, uint64_t pitch, uint64_t r
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Map of the output for tiles of 32 columns x 32 rows. False when TMA cannot store it (alignment).
+// Map of the output (16-byte aligned rows) for tiles of 32 columns x 32 rows.
 bool make_out_map(CUtensorMap* out, const Int8Params& p) {
   const uint64_t es = p.out_type == kOutF32 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(p.out) & 15) || (p.ldo * es) % 16 || p.ldo < p.N) return false;
   auto fn = int8_encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.N), static_cast<cuuint64_t>(p.M)};
@@ -1075,27 +1101,28 @@ int launch_stream(const CUtensorMap& mw, const CUtensorMap& mx, const Int8Params
 }
 
 // Which kernel runs a product: bt = 0 the persistent pairs, else the streaming kernel with bt tokens per tile and
-// `splits` CTAs per tile. The candidate with the least estimated cost wins. The estimate has a fixed part, a part per
-// 128 elements of K and one per token of the tile, times the share of an SM that a CTA gets; its constants are fitted
-// to the times of all candidates over M 1..4096 and eleven (K, N) from (300, 700) to (12288, 4096) so that the choice
-// is right (they are no times): the chosen candidate took 4 % longer than the best on average.
+// `splits` CTAs per tile. The candidate with the least estimated cost wins. An estimate has a fixed part, a part per
+// 128 elements of K and one per token of the tile, times the share of an SM that a CTA gets (pairs: the waves); its
+// constants are fitted to the times of all candidates over M 1..4096 and eleven (K, N) from (300, 700) to (12288,
+// 4096) so that the choice is right (they are no times): the chosen candidate took 3 % longer than the best on
+// average. `store_ok`: TMA can store the result (element stores cost the pairs another 6 us a wave at N = 1111).
 struct Int8Plan {
   int bt, splits;
 };
-Int8Plan plan_int8(int M, int N, int K, int sms) {
+Int8Plan plan_int8(int M, int N, int K, bool store_ok, int sms) {
   const int kbs = (K + kI8BK - 1) / kI8BK;
   const double pair_tiles = static_cast<double>((M + kI8Tile - 1) / kI8Tile) * ((N + kI8Tile - 1) / kI8Tile);
   const double waves = std::ceil(pair_tiles / (sms / 2));
-  double best = 14.3 + waves * kbs * 0.37 + (waves - 1) * 0.9;
+  double best = 11.5 + waves * kbs * 0.343 + (waves - 1) * 0.67 + (store_ok ? 0.0 : waves * 6.0);
   Int8Plan plan{0, 1};
-  for (int bt = 16; bt <= 128 && (bt == 16 || bt < 2 * M); bt *= 2) {
+  for (int bt = 16; bt <= kI8MaxTokens && (bt == 16 || bt < 2 * M); bt *= 2) {
     const double tiles = static_cast<double>((M + bt - 1) / bt) * ((N + kI8Rows - 1) / kI8Rows);
     for (int sp = 1; sp <= 8 && sp <= kbs; sp *= 2) {
       const double ctas = tiles * sp;
       if (sp > 1 && ctas > 4 * sms) break;
-      const double t = 6.3 + (sp > 1 ? 0.8 : 0.0) +
-                       (ctas > sms ? 2.1 * ctas / sms : 1.0) *
-                           (((kbs + sp - 1) / sp) * (0.155 + 0.00085 * bt) + 0.023 * bt);
+      const double t = 3.5 + (sp > 1 ? 0.6 : 0.0) +
+                       (ctas > sms ? 1.515 * ctas / sms : 1.0) *
+                           (((kbs + sp - 1) / sp) * (0.179 + 0.00148 * bt) + 0.0272 * bt);
       if (t < best) {
         best = t;
         plan = Int8Plan{bt, sp};
@@ -1221,7 +1248,10 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   p.in_type = in_type;
   p.status = status;
   p.w_early = w_early;
-  const Int8Plan plan = plan_int8(M, N, K, device_sm_count());
+  const int es = out_type == kOutF32 ? 4 : 2, rs = in_type == kOutF32 ? 4 : 2;
+  const bool store_ok = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo * es % 16 == 0 && ldo >= N &&
+                        (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && ldr * rs % 16 == 0));
+  const Int8Plan plan = plan_int8(M, N, K, store_ok, device_sm_count());
   CUtensorMap mx, mw, mo;
   if (plan.bt == 0) {
     p.tiles_m = (M + kI8Tile - 1) / kI8Tile;
@@ -1230,9 +1260,8 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
     if (static_cast<long long>(p.tiles_m) * p.tiles_n > 0x3fffffff) return -4;
     if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), 128)) return -7;
     if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), 128)) return -8;
-    const int rs = in_type == kOutF32 ? 4 : 2;
-    const bool res_ok = !residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * rs) % 16 == 0);
-    if (res_ok && make_out_map(&mo, p)) {
+    if (store_ok) {
+      if (!make_out_map(&mo, p)) return -9;
       if (out_type == kOutBf16) return launch_pair<kOutBf16, true>(mx, mw, mo, p, stream);
       if (out_type == kOutF16) return launch_pair<kOutF16, true>(mx, mw, mo, p, stream);
       return launch_pair<kOutF32, true>(mx, mw, mo, p, stream);
