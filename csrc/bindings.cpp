@@ -789,8 +789,8 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
   CHECK_CUDA(logits);
   TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf, "logits must be bf16 or fp16");
   auto f32 = [&](const at::Tensor& t, const char* name) -> const float* {
-    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == rows, name,
-                " must be contiguous float32 [rows]");
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == rows,
+                std::string(name) + " must be contiguous float32 [rows]");
     return t.data_ptr<float>();
   };
   const int* tk = nullptr;
@@ -809,20 +809,25 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
         "sample_counts");
 }
 
+// Refusals build their messages with this: streaming a number into a check's message crashes where the extension's
+// C++ runtime is not the one torch was built with.
+std::string num(int64_t v) { return std::to_string(v); }
+
 // x [rows, K] (pre 0: as it is, 1: RMSNorm with weight w, 2: SwiGLU of gate | up [rows, 2K]) -> int8 rows
 // q [rows, K rounded up to 16] and scale [rows], allocated when not given.
 std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w,
                                                  double eps, const c10::optional<at::Tensor>& q_out,
                                                  const c10::optional<at::Tensor>& scale_out, const at::Tensor& status) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be [rows, features]");
   const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
-  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be [rows, features], got ", x.sizes());
   const bool half = x.scalar_type() == at::kHalf;
-  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || (half && pre == 0), "x must be bfloat16",
-                    pre == 0 ? " or float16" : "", ", got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || (half && pre == 0), 
+                    std::string("x must be bfloat16") + (pre == 0 ? " or float16" : "") + ", got " +
+                        c10::toString(x.scalar_type()));
   TORCH_CHECK_VALUE(x.stride(1) == 1 || x.size(1) == 1, "the last dimension of x must be contiguous");
   TORCH_CHECK_VALUE(pre != 2 || x.size(1) % 2 == 0, "gate | up must be [rows, 2K]");
   const int64_t rows = x.size(0), K = pre == 2 ? x.size(1) / 2 : x.size(1), Kp = (K + 15) / 16 * 16;
-  TORCH_CHECK_VALUE(rows <= 0x7fffffff && K < 0x7fffff00, "too many rows or features: ", x.sizes());
+  TORCH_CHECK_VALUE(rows <= 0x7fffffff && K < 0x7fffff00, "too many rows or features");
   if (pre != 0) {
     const bool aligned = K % 8 == 0 && K <= 32768 && (rows <= 1 || x.stride(0) % 8 == 0) &&
                          reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
@@ -831,7 +836,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pr
   if (pre == 1) {
     TORCH_CHECK_VALUE(w.has_value() && w->numel() == K && w->is_contiguous() && w->device() == x.device() &&
                           w->scalar_type() == at::kBFloat16 && reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0,
-                      "the norm weight must be contiguous bfloat16 [", K, "] on x's device, aligned to 16 bytes");
+                      "the norm weight must be contiguous bfloat16 [" + num(K) + "] on x's device, aligned to 16 bytes");
   }
   at::Tensor q, scale;
   if (q_out.has_value()) {
@@ -839,8 +844,10 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pr
     scale = *scale_out;
     TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.is_contiguous() && q.dim() == 2 && q.size(0) == rows &&
                           q.size(1) == Kp && scale.scalar_type() == at::kFloat && scale.is_contiguous() &&
-                          scale.numel() == rows && q.device() == x.device() && scale.device() == x.device(),
-                      "out does not hold ", rows, " x ", K, " int8 rows on ", x.device());
+                          scale.numel() == rows && q.device() == x.device() && scale.device() == x.device() &&
+                          reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+                      "out does not hold " + num(rows) + " x " + num(K) + " int8 rows on " + x.device().str() +
+                          ", aligned to 16 bytes");
   } else {
     q = at::empty({rows, Kp}, x.options().dtype(at::kChar));
     scale = at::empty({rows}, x.options().dtype(at::kFloat));
@@ -866,10 +873,10 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
   const int64_t M = qx.size(0), N = qw.size(0), Kp = (K + 15) / 16 * 16;
   const auto dev = qw.device();
   auto on_device = [&](const at::Tensor& t) {
-    TORCH_CHECK_VALUE(t.device() == dev, "every tensor must be on the weight's device ", dev, ", got one on ", t.device());
+    TORCH_CHECK_VALUE(t.device() == dev, "every tensor must be on the weight's device " + dev.str() + ", got one on " + t.device().str());
   };
   on_device(qx), on_device(sx), on_device(sw);
-  TORCH_CHECK_VALUE(K > 0 && K <= 133144, "in must be at most 133144, got ", K);
+  TORCH_CHECK_VALUE(K > 0 && K <= 133144, "in must be at most 133144, got " + num(K));
   for (const at::Tensor* q : {&qx, &qw})
     TORCH_CHECK_VALUE(q->scalar_type() == at::kChar && q->dim() == 2 && q->is_contiguous() && q->size(1) == Kp &&
                           reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 == 0,
@@ -883,7 +890,7 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
     out = *out_opt;
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == M && out.size(1) == N && float_type_id(out.scalar_type()) >= 0 &&
                           (N <= 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N),
-                      "out must be bf16, fp16 or fp32 [", M, ", ", N, "] with a contiguous last dimension");
+                      "out must be bf16, fp16 or fp32 [" + num(M) + ", " + num(N) + "] with a contiguous last dimension");
     on_device(out);
   } else {
     TORCH_CHECK_VALUE(out_dtype.has_value() && float_type_id(*out_dtype) >= 0, "out_dtype must be bf16, fp16 or fp32");
@@ -894,7 +901,7 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
   if (residual.has_value()) {
     TORCH_CHECK_VALUE(residual->dim() == 2 && residual->size(0) == M && residual->size(1) == N &&
                           float_type_id(residual->scalar_type()) >= 0 && (N <= 1 || residual->stride(1) == 1),
-                      "residual must be bf16, fp16 or fp32 [", M, ", ", N, "] with a contiguous last dimension");
+                      "residual must be bf16, fp16 or fp32 [" + num(M) + ", " + num(N) + "] with a contiguous last dimension");
     on_device(*residual);
     in_type = float_type_id(residual->scalar_type());
     ldr = residual->stride(0);
@@ -902,7 +909,7 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
   if (bias.has_value()) {
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->numel() == N && bias->is_contiguous() &&
                           float_type_id(bias->scalar_type()) >= 0,
-                      "bias must be contiguous bf16, fp16 or fp32 [", N, "]");
+                      "bias must be contiguous bf16, fp16 or fp32 [" + num(N) + "]");
     on_device(*bias);
     TORCH_CHECK_VALUE(!residual.has_value() || bias->scalar_type() == residual->scalar_type(),
                       "bias and residual must be of one type");
@@ -921,9 +928,8 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& qw, const at::Tens
                        const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
                        const c10::optional<at::Tensor>& out, const c10::optional<at::ScalarType>& out_dtype,
                        const at::Tensor& status) {
-  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "inner dimensions differ (", x.sizes(), " vs ", K, ")");
-  TORCH_CHECK_VALUE(x.device() == qw.device(), "every tensor must be on the weight's device ", qw.device(),
-                    ", got one on ", x.device());
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "inner dimensions differ (x needs " + num(K) + " columns)");
+  TORCH_CHECK_VALUE(x.device() == qw.device(), "every tensor must be on the weight's device " + qw.device().str() + ", got one on " + x.device().str());
   auto [qx, sx] = quantize_rows(x, 0, c10::nullopt, 0.0, c10::nullopt, c10::nullopt, status);
   if (g_last_rc != 0) return qx;  // reported by the caller
   return gemm_int8(qx, sx, qw, sw, K, bias, residual, out, out_dtype.has_value() ? out_dtype : x.scalar_type(), status,

@@ -469,20 +469,24 @@ ACCERL_DEVINL void store_from_float(void* p, long long i, int type, float v) {
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
-// Four neighbouring channels of a row: y = acc * sx * sw + bias (+ residual).
+// Four neighbouring channels of a row: the residual as it is loaded, and y = acc * sx * sw + bias (+ residual).
+ACCERL_DEVINL uint4 load_residual4(const Int8Params& p, long long t, int n) {
+  if (!p.residual) return make_uint4(0, 0, 0, 0);
+  const long long at = t * p.ldr + n;
+  if (p.in_type == kOutF32) return *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.residual) + at);
+  const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p.residual) + at);
+  return make_uint4(r.x, r.y, 0, 0);
+}
 template <int OUT>
-ACCERL_DEVINL void finish4(const Int8Params& p, long long t, int n, int4 acc, float sx, float4 sw, float4 b) {
+ACCERL_DEVINL void finish4(const Int8Params& p, long long t, int n, int4 acc, float sx, float4 sw, float4 b, uint4 r) {
   float4 y = make_float4(__fmaf_rn(static_cast<float>(acc.x), sx * sw.x, b.x),
                          __fmaf_rn(static_cast<float>(acc.y), sx * sw.y, b.y),
                          __fmaf_rn(static_cast<float>(acc.z), sx * sw.z, b.z),
                          __fmaf_rn(static_cast<float>(acc.w), sx * sw.w, b.w));
   if (p.residual) {
-    const long long at = t * p.ldr + n;
     if (p.in_type == kOutF32) {
-      const float4 r = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + at);
-      y.x += r.x, y.y += r.y, y.z += r.z, y.w += r.w;
+      y.x += __uint_as_float(r.x), y.y += __uint_as_float(r.y), y.z += __uint_as_float(r.z), y.w += __uint_as_float(r.w);
     } else {
-      const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p.residual) + at);
       const bool bf = p.in_type == kOutBf16;
       const float2 lo = bf ? Half16<__nv_bfloat16>::unpack(r.x) : Half16<__half>::unpack(r.x);
       const float2 hi = bf ? Half16<__nv_bfloat16>::unpack(r.y) : Half16<__half>::unpack(r.y);
@@ -664,15 +668,24 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
   if constexpr (VEC) {
     const int n = n0 + lane * 4;
     if (n < p.N) {  // N is a multiple of 4
-#pragma unroll 4
-      for (int c = c_lo + warp; c < c_hi; c += kWarps) {
-        const int4* src = reinterpret_cast<const int4*>(parts + (c - c_lo) * kI8Rows) + lane;
-        int4 acc = *src;
-        for (int r = 1; r < splits; ++r) {
-          const int4 o = src[r * share * (kI8Rows / 4)];
-          acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+      constexpr int kRows = 4;  // tokens at once: their residuals are loaded before any result is stored
+      for (int c0 = c_lo + warp; c0 < c_hi; c0 += kWarps * kRows) {
+        uint4 res[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (c0 + i * kWarps < c_hi) res[i] = load_residual4(p, t0 + c0 + i * kWarps, n);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int c = c0 + i * kWarps;
+          if (c >= c_hi) break;
+          const int4* src = reinterpret_cast<const int4*>(parts + (c - c_lo) * kI8Rows) + lane;
+          int4 acc = *src;
+          for (int r = 1; r < splits; ++r) {
+            const int4 o = src[r * share * (kI8Rows / 4)];
+            acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+          }
+          finish4<OUT>(p, t0 + c, n, acc, sx_s[c], sw, b, res[i]);
         }
-        finish4<OUT>(p, t0 + c, n, acc, sx_s[c], sw, b);
       }
     }
   } else {
@@ -683,19 +696,32 @@ __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __gr
       sc[i] = n < p.N ? p.sw[n] : 0.f;
       bi[i] = (n < p.N && p.bias) ? load_as_float(p.bias, n, p.in_type) : 0.f;
     }
-    for (int c = c_lo + warp; c < c_hi; c += kWarps) {
-      const long long t = t0 + c;
-      const float sx = sx_s[c];
+    constexpr int kRows = 4;
+    for (int c0 = c_lo + warp; c0 < c_hi; c0 += kWarps * kRows) {
+      float res[kRows][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = n0 + i * 32 + lane;
-        if (n >= p.N) continue;
-        const int* src = parts + (c - c_lo) * kI8Rows + i * 32 + lane;
-        int acc = *src;
-        for (int r = 1; r < splits; ++r) acc += src[r * share * kI8Rows];
-        float y = __fmaf_rn(static_cast<float>(acc), sx * sc[i], bi[i]);
-        if (p.residual) y += load_as_float(p.residual, t * p.ldr + n, p.in_type);
-        store_from_float(p.out, t * p.ldo + n, OUT, y);
+      for (int j = 0; j < kRows; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = c0 + j * kWarps, n = n0 + i * 32 + lane;
+          res[j][i] = p.residual && c < c_hi && n < p.N
+                          ? load_as_float(p.residual, static_cast<long long>(t0 + c) * p.ldr + n, p.in_type)
+                          : 0.f;
+        }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int c = c0 + j * kWarps;
+        if (c >= c_hi) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = n0 + i * 32 + lane;
+          if (n >= p.N) continue;
+          const int* src = parts + (c - c_lo) * kI8Rows + i * 32 + lane;
+          int acc = *src;
+          for (int r = 1; r < splits; ++r) acc += src[r * share * kI8Rows];
+          store_from_float(p.out, static_cast<long long>(t0 + c) * p.ldo + n, OUT,
+                           __fmaf_rn(static_cast<float>(acc), sx_s[c] * sc[i], bi[i]) + res[j][i]);
+        }
       }
     }
   }
@@ -1116,6 +1142,7 @@ Int8Plan plan_int8(int M, int N, int K, bool store_ok, int sms) {
   double best = 11.5 + waves * kbs * 0.343 + (waves - 1) * 0.67 + (store_ok ? 0.0 : waves * 6.0);
   Int8Plan plan{0, 1};
   for (int bt = 16; bt <= kI8MaxTokens && (bt == 16 || bt < 2 * M); bt *= 2) {
+    if ((M + bt - 1) / bt > 65535) continue;  // a grid's second dimension
     const double tiles = static_cast<double>((M + bt - 1) / bt) * ((N + kI8Rows - 1) / kI8Rows);
     for (int sp = 1; sp <= 8 && sp <= kbs; sp *= 2) {
       const double ctas = tiles * sp;
@@ -1273,7 +1300,6 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   }
   p.bt = plan.bt;
   const dim3 grid((N + kI8Rows - 1) / kI8Rows, (M + p.bt - 1) / p.bt, plan.splits);
-  if (grid.y > 65535) return -4;
   const int kbs = (K + kI8BK - 1) / kI8BK;
   const int stage_bytes = (kI8Rows + p.bt) * kI8BK;
   // the accumulator: behind the stages where peers write it, else where the stages were

@@ -6,6 +6,7 @@ bf16 on the GPU: tilings of the attention).
 """
 
 import asyncio
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -50,13 +51,18 @@ def generate(eng, prompts, params):
     return [o.outputs[0] for o in asyncio.run(run())]
 
 
-def int8_projections(monkeypatch, cfg):
-    """Replace the layers' products by 8-bit ones (the LM head stays)."""
+def int8_projections(monkeypatch, cfg, tp=1):
+    """Replace the layers' products by 8-bit ones (the LM head stays); with ``tp`` ranks a row-parallel weight
+    (hidden_size rows) and its input are quantised shard by shard."""
     plain = ops.linear
 
     def linear(x, w, bias=None, residual=None, out=None):
         if w.shape[0] == cfg.vocab_size:
             return plain(x, w, bias, residual, out)
+        if tp > 1 and w.shape[0] == cfg.hidden_size:
+            parts = [ops.linear_int8(ops.quantize_rows(xs.contiguous()), ops.quantize_rows(ws.contiguous()),
+                                     out_dtype=x.dtype) for xs, ws in zip(x.chunk(tp, 1), w.chunk(tp, 1))]
+            return sum(parts) + residual
         return ops.linear_int8(ops.quantize_rows(x.contiguous()), ops.quantize_rows(w), bias, residual, out,
                                None if out is not None else x.dtype)
 
@@ -229,3 +235,85 @@ def test_uniform_numbers():
     assert np.array_equal(u[100:110], uniform_numbers(seeds[100:110], pos[100:110]))
     counts = np.histogram(u, 16, (0, 1))[0]
     assert np.abs(counts - 256).max() <= 5 * 240 ** 0.5
+
+
+def _tp_rank(rank, port, q):
+    """One of two ranks of a tensor-parallel engine with 8-bit shards; the leader's outputs, and those of a second
+    pass after the weights changed, go to ``q``."""
+    import os
+    import traceback
+
+    import torch.distributed as dist
+
+    try:
+        os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+        dist.init_process_group("gloo", rank=rank, world_size=2)
+        cmd = dist.new_group(backend="gloo")
+        cfg = get_preset("tiny-qwen2")
+        cfg.vocab_size = 512
+        m = build_model(cfg, "full", torch.device("cpu"), torch.float32, with_grads=False)
+        m.init_weights(seed=11, std=0.08)
+        eng = GenerationEngine(cfg, torch.device("cpu"), torch.float32, max_num_seqs=8, max_num_batched_tokens=64,
+                               num_blocks=64, block_size=4, tp_group=dist.group.WORLD, cmd_group=cmd,
+                               quantization="int8")
+        eng.set_weight_source(m.layout, tensor=m.params)
+        if rank == 0:
+            results = []
+            for scale in (1.0, 1.2):
+                m.params.mul_(scale)
+                eng.pull_weights("all")
+                eng.allocator.clear_cache()  # keys and values of the old weights, as the service's pause clears them
+                results.append([(o, lps) for o, lps in generate_without_shutdown(eng, PROMPTS[:2], f"t{scale}")])
+            asyncio.run(eng.shutdown())
+            eng.stop_followers()
+            q.put(results)
+        else:
+            m.params.mul_(1.0)
+            original = eng._pull_local
+
+            def pull(scope, calls=[0]):
+                if calls[0] == 1:
+                    m.params.mul_(1.2)
+                calls[0] += 1
+                return original(scope)
+
+            eng._pull_local = pull
+            eng.serve_follower()
+            name = "model.layers.0.mlp.down_proj.weight"
+            expect = ops.quantize_rows(eng.model.w(name))
+            q.put(bool(torch.equal(eng._w8[name].q, expect.q) and torch.equal(eng._w8[name].scale, expect.scale)))
+        dist.destroy_process_group()
+    except Exception:  # pragma: no cover
+        q.put(traceback.format_exc())
+
+
+def test_int8_tensor_parallel_cpu(monkeypatch):
+    """Two ranks, each with its own shards in 8 bits (row-parallel weights get a scale per channel and shard), before
+    and after a weight update, against the recomputation with the same shards."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    queue = ctx.Queue()
+    procs = [ctx.Process(target=_tp_rank, args=(r, port, queue)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = [queue.get(timeout=240) for _ in procs]
+    for p in procs:
+        p.join(60)
+    assert not any(isinstance(g, str) for g in got), [g for g in got if isinstance(g, str)]
+    assert True in got  # the follower's copies follow its weights
+    tp = next(g for g in got if isinstance(g, list))
+    cfg = get_preset("tiny-qwen2")
+    cfg.vocab_size = 512
+    m = build_model(cfg, "full", torch.device("cpu"), torch.float32, with_grads=False)
+    m.init_weights(seed=11, std=0.08)
+    int8_projections(monkeypatch, cfg, tp=2)
+    for scale, outs in zip((1.0, 1.2), tp):
+        m.params.mul_(scale)
+        got = [SimpleNamespace(token_ids=toks, logprobs=[{t: v[0]} for t, v in zip(toks, lps)]) for toks, lps in outs]
+        check_greedy(m, PROMPTS, got, 0.05)

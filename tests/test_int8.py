@@ -308,6 +308,36 @@ def test_refusals_gpu():
 
 
 @pytest.mark.gpu
+def test_misaligned_rows_are_refused_or_taken():
+    """Buffers that do not start on 16 bytes: int8 rows are refused, everything else is taken element by element."""
+    buf = torch.zeros(4 * 64 + 64, dtype=torch.int8, device="cuda")
+    q = buf[3 : 3 + 4 * 64].view(4, 64)
+    x = randn(4, 64, device="cuda")
+    w = ops.quantize_rows(randn(8, 64, seed=1, device="cuda"))
+    with pytest.raises(ValueError, match="aligned"):
+        ops.quantize_rows(x, out=ops.Int8Rows(q, torch.zeros(4, device="cuda"), 64))
+    with pytest.raises(ValueError, match="aligned"):
+        ops.linear_int8(ops.Int8Rows(q, torch.zeros(4, device="cuda"), 64), w)
+    r = ops.quantize_rows(x)
+    scales = torch.zeros(9, device="cuda")
+    scales[1:] = w.scale
+    bias = randn(9, seed=2, device="cuda")[1:]
+    shifted = ops.Int8Rows(w.q, scales[1:], 64)
+    check_product(ops.linear_int8(r, shifted, bias=bias), *product64(r, w, bias))
+
+
+@pytest.mark.gpu
+def test_many_rows():
+    """More rows than a grid's second dimension holds of the smallest tile, and a broadcast residual."""
+    m, k, n = 1_100_000, 16, 8
+    x = randn(m, k, device="cuda")
+    w = ops.quantize_rows(randn(n, k, seed=1, device="cuda"))
+    r = ops.quantize_rows(x)
+    res = randn(1, n, seed=2, device="cuda").expand(m, -1)
+    check_product(ops.linear_int8(r, w, residual=res), *product64(r, w, None, res))
+
+
+@pytest.mark.gpu
 def test_linear_int8_in_a_graph_and_on_another_stream():
     """Capture with fixed buffers, then replay on new inputs; and the same call on a side stream."""
     for m, k, n in ((4, 1536, 2048), (300, 512, 640), (1024, 1536, 1024)):
