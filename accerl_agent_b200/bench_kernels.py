@@ -266,6 +266,29 @@ def bench_decode(results):
         torch.cuda.empty_cache()
 
 
+def bench_int8(results):
+    """8-bit linear layers (rows to int8 and product, as ``ops.linear_int8`` runs them) next to the bf16 layer on
+    the 1.5B shape, and sampling from given numbers on its vocabulary."""
+    peak_tf, peak_gbs = _peaks()
+    for M, K, N in ((1, 1536, 2048), (64, 1536, 17920), (256, 8960, 1536), (8192, 1536, 17920), (8192, 8960, 1536)):
+        x = torch.randn(M, K, device="cuda").bfloat16()
+        w = (torch.randn(N, K, device="cuda") * 0.02).bfloat16()
+        w8 = ops.quantize_rows(w)
+        t8 = median_ms(lambda: ops.linear_int8(x, w8))
+        t16 = median_ms(lambda: ops.linear(x, w))
+        flops, nbytes = 2.0 * M * N * K, 2 * M * K + N * K + 2 * M * N
+        results[f"int8/{M}x{K}x{N}"] = {"ms": t8, "tflops": flops / t8 / 1e9, "gbs": nbytes / t8 / 1e6, "bf16_ms": t16,
+                                        "floor_ms": max(flops / (2 * peak_tf) / 1e9, nbytes / peak_gbs / 1e6)}
+        del x, w, w8
+    for rows, V in ((1, 151936), (64, 151936), (256, 151936)):
+        logits = (torch.randn(rows, V, device="cuda") * 2.5).bfloat16()
+        u = torch.rand(rows, device="cuda")
+        temp, top_p = torch.full((rows,), 0.8, device="cuda"), torch.full((rows,), 0.95, device="cuda")
+        t = median_ms(lambda: ops.sample_inverse_cdf(logits, u, temp, top_p=top_p))
+        results[f"sample_inverse_cdf/{rows}x{V}"] = {"ms": t, "gbs": 2 * rows * V / t / 1e6,
+                                                     "frac_hbm": 2 * rows * V / t / 1e6 / peak_gbs}
+
+
 PROFILE_CASES = ("attnprof", "gemmprof", "moeprof", "opsprof", "decodeprof")
 
 
@@ -293,6 +316,8 @@ def main():
         bench_memory_bound(results)
     if "decode" in sel:
         bench_decode(results)
+    if "int8" in sel:
+        bench_int8(results)
     for k, v in results.items():
         if isinstance(v, dict) and "tflops" in v:
             v["frac_of_measured_peak"] = v["tflops"] / peak_tf
