@@ -172,6 +172,9 @@ struct CountShared {
   double cum;                                 // mass up to and with that token
   int nth_here;                               // rank of the drawn token within this CTA's slice, or -1
   float logprob;
+  float set_t, set_u, set_p, set_min;         // the row's settings
+  int set_k;
+  uint32_t left_out;                          // counts nothing of use
 };
 
 // a count as a 64-bit float without the slow conversion
@@ -207,7 +210,8 @@ struct RowWeights {
   ACCERL_DEVINL double mass(uint32_t key, double sc) const {
     // an infinite maximum leaves nothing to the others (whose gap is -inf); at an infinite temperature (sc = 0)
     // every finite gap weighs 1
-    const double w = exp2_64th(fmax(gap(key) * sc, -64.0 * 1021), table);
+    const double y = gap(key) * sc;
+    const double w = exp2_64th(y > -64.0 * 1021 ? y : -64.0 * 1021, table);  // NaN (inf * 0): the limit
     return key == max_key ? 1.0 : (isinf(max) ? 0.0 : w);
   }
   ACCERL_DEVINL double weight(uint32_t key) const { return mass(key, scale); }
@@ -219,15 +223,19 @@ struct RowWeights {
       // `above` of the keys lie above the maximum and hold nothing
       const uint32_t above = key[3] > max_key ? min(key[3] - max_key, 4u) : 0u;
       const double m0 = mass(key[3] - above, sc), r2 = r * r;
-      const double m[4] = {m0, m0 * r, m0 * r2, (m0 * r) * r2};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {  // key[j] is 3 - j - above steps below the first
-        const uint32_t d = 3u - j;
-        w[j] = d < above ? 0.0 : (d - above == 0u ? m[0] : d - above == 1u ? m[1] : d - above == 2u ? m[2] : m[3]);
+      w[3] = m0;
+      w[2] = m0 * r;
+      w[1] = m0 * r2;
+      w[0] = w[2] * r2;
+      for (uint32_t i = 0; i < above; ++i) {  // only where the maximum is
+        w[0] = w[1];
+        w[1] = w[2];
+        w[2] = w[3];
+        w[3] = 0.0;
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = mass(key[j], sc);
+      for (int j = 0; j < 4; ++j) w[j] = key[j] > max_key ? 0.0 : mass(key[j], sc);
     }
   }
   ACCERL_DEVINL bool kept(uint32_t key, double w) const { return key == max_key || !(min_p > 0.0) || w >= min_p; }
@@ -255,42 +263,37 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
   const int per = (chunks + csize - 1) / csize;
   const int ch0 = min(chunks, rank * per), ch1 = min(chunks, ch0 + per);
   // chunk ch of the row; elements outside it read as NaN, which nothing counts
+  auto load2 = [&](int ch, int j) -> uint32_t {  // two elements of it
+    const int a = ch * 8 - head + 2 * j, b = a + 1;
+    const uint32_t lo = (a >= 0 && a < V) ? x[a] : 0xffffu, hi = (b >= 0 && b < V) ? x[b] : 0xffffu;
+    return lo | (hi << 16);
+  };
   auto load8 = [&](int ch) -> uint4 {
     const int i0 = ch * 8 - head;
     if (i0 >= 0 && i0 + 8 <= V) return *reinterpret_cast<const uint4*>(x + i0);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int a = i0 + 2 * j, b = a + 1;
-      const uint32_t lo = (a >= 0 && a < V) ? x[a] : 0xffffu, hi = (b >= 0 && b < V) ? x[b] : 0xffffu;
-      w[j] = lo | (hi << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(load2(ch, 0), load2(ch, 1), load2(ch, 2), load2(ch, 3));
   };
   // chunks [whole0, whole1) lie inside the row
   const int whole0 = head ? 1 : 0, whole1 = (head + V) / 8;
   constexpr int kAhead = 2;
   const uint4* src = reinterpret_cast<const uint4*>(x - head);
-  // this thread's kAhead chunks from c on; behind `end` NaN, which nothing counts
+  // this thread's kAhead whole chunks from c on; behind `end` NaN, which nothing counts
   auto load_batch = [&](uint4 (&v)[kAhead], int c, int end) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int ch = c + j * kCntThreads;
-      v[j] = ch >= whole0 && ch < min(end, whole1) ? __ldg(src + ch) : make_uint4(~0u, ~0u, ~0u, ~0u);
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {  // the row's ends
-      const int ch = c + j * kCntThreads;
-      if (ch < end && (ch < whole0 || ch >= whole1)) v[j] = load8(ch);
+      v[j] = ch < end ? __ldg(src + ch) : make_uint4(~0u, ~0u, ~0u, ~0u);
     }
   };
+  auto load_first = [&](uint4 (&v)[kAhead], int a, int b) { load_batch(v, max(a, whole0) + tid, min(b, whole1)); };
   // f(word) for every two elements of the chunks [a, b), the next batch on its way while one is worked on; `v`
-  // holds the first
+  // holds the first. The row's ends, which are not whole chunks, come after the loop: it has no other tests.
   auto for_each = [&](uint4 (&v)[kAhead], int a, int b, auto f) {
+    const int end = min(b, whole1);
 #pragma unroll 1
-    for (int c = a + tid; c < b; c += kAhead * kCntThreads) {
+    for (int c = max(a, whole0) + tid; c < end; c += kAhead * kCntThreads) {
       uint4 next[kAhead];
-      load_batch(next, c + kAhead * kCntThreads, b);
+      load_batch(next, c + kAhead * kCntThreads, end);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         f(v[j].x);
@@ -299,6 +302,10 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
         f(v[j].w);
         v[j] = next[j];
       }
+    }
+    if (tid < 8) {  // a word each
+      const int ch = tid < 4 ? 0 : whole1;  // the same one where the row ends in its first chunk
+      if (ch >= a && ch < b && (tid < 4 ? whole0 == 1 : whole1 < chunks && whole1 >= whole0)) f(load2(ch, tid & 3));
     }
   };
   auto valid_key = [](uint32_t w) -> int {  // -1: -inf or NaN
@@ -309,38 +316,34 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     for (int i = tid; i < static_cast<int>((kBins + 64) / 4); i += kCntThreads) dyn[i] = make_uint4(0, 0, 0, 0);
   };
   auto add = [&](uint32_t bin) { atomicAdd(&hist[bin], 1u); };
-  // the same under a predicate, not a branch
-  const uint32_t hist_smem = smem_u32(hist);
+  // the same with a select, not a branch: what is left out goes to one word, which the hardware adds up per warp
+  const uint32_t hist_smem = smem_u32(hist), left_out = smem_u32(&sh.left_out);
   auto add_unless = [&](uint32_t skip, uint32_t bin) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.eq.u32 p, %1, 0;\n"
-        "@p red.shared::cta.add.u32 [%0], 1;\n"
-        "}\n" ::"r"(hist_smem + bin * 4u),
-        "r"(skip)
-        : "memory");
+    const uint32_t at = skip ? left_out : hist_smem + bin * 4u;
+    asm volatile("red.shared::cta.add.u32 [%0], 1;" ::"r"(at) : "memory");
   };
 
-  // the row's settings, on their way while the slice is counted
-  const float t = temperature[row], row_u = u[row];
-  const float row_p = top_p ? top_p[row] : 1.f, row_min = min_p ? min_p[row] : 0.f;
-  const int row_k = top_k ? top_k[row] : 0;
   // the first loads travel while the counters are cleared
   uint4 batch[kAhead];
-  load_batch(batch, ch0 + tid, ch1);
+  load_first(batch, ch0, ch1);
   __syncwarp();
   cluster_arrive_relaxed();
   clear();
   if (tid < 3) sh.found[tid] = kCntGroups;
   if (tid == 0) sh.nth_here = -1;
-  const bool greedy = !(t > 0.f);
-  const double td = greedy ? 1.0 : static_cast<double>(t);
+  if (tid == 192) {  // the row's settings, out of the registers while the slice is counted
+    sh.set_t = temperature[row];
+    sh.set_u = u[row];
+    sh.set_p = top_p ? top_p[row] : 1.f;
+    sh.set_min = min_p ? min_p[row] : 0.f;
+    sh.set_k = top_k ? top_k[row] : 0;
+  }
   if (tid < 64) sh.exp2_table[tid] = exp2(tid / 64.0);
   if (tid >= 64 && tid < 192 && ((tid - 64) & 63) < static_cast<int>(S >> Key16<T>::kMantissa)) {
     const uint32_t first = Key16<T>::kBase + (((tid - 64) & 63) << Key16<T>::kMantissa);
     const double step = static_cast<double>(Key16<T>::value(first + 1) - Key16<T>::value(first));
-    sh.ratio[(tid - 64) >> 6][(tid - 64) & 63] = exp(-step / (tid < 128 ? td : 1.0));
+    const float t = tid < 128 ? temperature[row] : 1.f;
+    sh.ratio[(tid - 64) >> 6][(tid - 64) & 63] = exp(-step / (t > 0.f ? static_cast<double>(t) : 1.0));
   }
   __syncthreads();
 
@@ -360,16 +363,16 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     low2 |= Key16<T>::below(t);
   });
   uint32_t escape = 0;
-  if (low2 & 0x80008000u) {  // zeros, or magnitudes below the window
-    for (int c = ch0 + tid; c < ch1; c += kCntThreads) {
-      const uint4 q = load8(c);
-      const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t mag = (qw[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
+  if (low2 & 0x80008000u) {  // zeros, or magnitudes below the window, among the elements this thread has seen
+    load_first(batch, ch0, ch1);
+    for_each(batch, ch0, ch1, [&](uint32_t w) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t mag = (w >> (16 * h)) & 0x7fffu;
         if (mag == 0u) add(0u);
         else if (static_cast<int>(mag) < static_cast<int>(Key16<T>::kBase)) escape = 1u;
       }
-    }
+    });
   }
   // the largest and the smallest of both halves as keys (0: there is nothing but NaN)
   auto one_key = [](uint32_t bits) -> uint32_t {
@@ -414,6 +417,9 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     any_low |= sh.any_low[c];
     escape |= sh.escape[c];
   }
+  const float t = sh.set_t, row_min = sh.set_min;
+  const bool greedy = !(t > 0.f);
+  const double td = greedy ? 1.0 : static_cast<double>(t);
   RowWeights<T> rw;
   rw.scale = kLog2e64 / td;
   rw.table = sh.exp2_table;
@@ -434,27 +440,30 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     // neighbouring pairs of groups, which are either all populated or all empty, to different CTAs
     for (int i2 = warp * csize + rank; i2 * 2 < n; i2 += csize * kCntWarps) {
       const uint32_t b0 = static_cast<uint32_t>(i2) * 128 + lane * 4;
-      uint32_t c[4] = {0, 0, 0, 0};
+      const uint4 own = *reinterpret_cast<const uint4*>(hist + b0);
+      uint32_t c[4] = {own.x, own.y, own.z, own.w};
+      if (csize > 1) {
 #pragma unroll
-      for (int r = 0; r < kCntMaxCluster; ++r)
-        if (r < csize) {
-          const uint4 v = *reinterpret_cast<const uint4*>(peer(hist, r) + b0);
-          c[0] += v.x;
-          c[1] += v.y;
-          c[2] += v.z;
-          c[3] += v.w;
-        }
+        for (int r = 1; r < kCntMaxCluster; ++r)
+          if (r < csize) {  // csize is a power of two
+            const uint4 v = *reinterpret_cast<const uint4*>(peer(hist, rank ^ r) + b0);
+            c[0] += v.x;
+            c[1] += v.y;
+            c[2] += v.z;
+            c[3] += v.w;
+          }
+      }
       uint32_t num = 0;
       double m = 0.0;
       if (__any_sync(0xffffffffu, (c[0] | c[1] | c[2] | c[3]) != 0u)) {
         // the leader's counters of these bins, which nobody else reads, take the whole cluster's counts
         if (csize > 1) *reinterpret_cast<uint4*>(peer(hist, 0) + b0) = make_uint4(c[0], c[1], c[2], c[3]);
-        uint32_t key[4];
         double w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) key[j] = key_of(b0 + j);
+        // four neighbours, but in the group of zero, which has one value
+        const uint32_t key0 = key_of(b0), step = slow || b0 >= 64u ? 1u : 0u;
+        const uint32_t key[4] = {key0, key0 + step, key0 + 2u * step, key0 + 3u * step};
         // the slow path's keys lie anywhere: no table
-        const bool even = !slow && key[3] - key[0] == 3u;
+        const bool even = !slow && step != 0u;
         const uint32_t binade = even ? ((key_bits(key[3]) & 0x7fffu) - Key16<T>::kBase) >> Key16<T>::kMantissa : 0u;
         auto take = [&](const double (&at_t)[4], const double (&at_1)[4]) {
           double mk[4], ml[4];
@@ -462,8 +471,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
           for (int j = 0; j < 4; ++j) {
             const uint32_t k = rw.kept(key[j], at_t[j]) ? c[j] : 0u;
             num += k;
-            mk[j] = k ? count_f64(k) * at_t[j] : 0.0;
-            ml[j] = c[j] ? count_f64(c[j]) * at_1[j] : 0.0;
+            mk[j] = count_f64(k) * at_t[j];  // a weight is finite
+            ml[j] = count_f64(c[j]) * at_1[j];
           }
           m = (mk[0] + mk[1]) + (mk[2] + mk[3]);
           lse += (ml[0] + ml[1]) + (ml[2] + ml[3]);
@@ -502,7 +511,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       cluster_sync();  // the window before has been read
       clear();
       __syncthreads();
-      load_batch(batch, ch0 + tid, ch1);
+      load_first(batch, ch0, ch1);
       for_each(batch, ch0, ch1, [&](uint32_t w) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -536,45 +545,55 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       }
       return bits;
     };
-    // each warp counts a contiguous part; the one that holds the token goes through its part again
-    const int wper = (b - a + kCntWarps - 1) / kCntWarps;
-    const int w0 = min(b, a + warp * wper), w1 = min(b, w0 + wper);
-    uint32_t n = 0;
+    // The CTA counts strip after strip until one holds the token, each warp a contiguous part; the warp that has it
+    // goes through its part again. (256 rows of 151936: half of the row on average, 9 us of them for 13.)
     constexpr int kBatch = 8;
-    for (int c = w0 + lane; c < w1; c += 32 * kBatch) {
+    const int wper = min(32 * kBatch, (b - a + kCntWarps - 1) / kCntWarps);
+    uint32_t base = 0;
+    int parity = 0;
+#pragma unroll 1
+    for (int s0 = a; s0 < b; s0 += wper * kCntWarps, parity ^= 1) {
+      const int w0 = min(b, s0 + warp * wper), w1 = min(b, w0 + wper);
+      uint32_t n = 0;
       uint4 v[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int ch = c + 32 * j;
+        const int ch = w0 + lane + 32 * j;
         v[j] = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN is no candidate's pattern
         if (ch < w1 && ch >= whole0 && ch < whole1) v[j] = __ldg(src + ch);
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int ch = c + 32 * j;
+        const int ch = w0 + lane + 32 * j;
         if (ch < w1 && (ch < whole0 || ch >= whole1)) v[j] = load8(ch);
       }
       Key16<T>::count_equal(v, want * 0x00010001u, n);
-    }
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sh.warp_u[0][warp] = n;
-    __syncthreads();
-    uint32_t at = 0;
-    for (int w = 0; w < warp; ++w) at += sh.warp_u[0][w];
-    if (nth < at || nth >= at + n) return;
-    for (int c0 = w0; c0 < w1; c0 += 32) {
-      const uint32_t bits = c0 + lane < w1 ? matches(load8(c0 + lane)) : 0u;
-      const uint32_t mine = __popc(bits);
-      const uint32_t incl = warp_scan_u32(mine, lane);
-      const uint32_t excl = at + incl - mine;
-      if (nth >= excl && nth < excl + mine) {
-        uint32_t left = bits;
-        for (uint32_t i = excl; i < nth; ++i) left &= left - 1;
-        out_tokens[row] = static_cast<long long>(c0 + lane) * 8 - head + __ffs(left) - 1;
-        out_logprobs[row] = lp;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) sh.warp_u[parity][warp] = n;
+      __syncthreads();
+      const uint32_t count = lane < kCntWarps ? sh.warp_u[parity][lane] : 0u;
+      const uint32_t total = __reduce_add_sync(0xffffffffu, count);
+      if (nth >= base + total) {
+        base += total;
+        continue;
       }
-      at += __shfl_sync(0xffffffffu, incl, 31);
-      if (nth < at) break;
+      uint32_t at = base + __reduce_add_sync(0xffffffffu, lane < warp ? count : 0u);
+      if (nth < at || nth >= at + n) return;
+      for (int c0 = w0; c0 < w1; c0 += 32) {
+        const uint32_t bits = c0 + lane < w1 ? matches(load8(c0 + lane)) : 0u;
+        const uint32_t mine = __popc(bits);
+        const uint32_t incl = warp_scan_u32(mine, lane);
+        const uint32_t excl = at + incl - mine;
+        if (nth >= excl && nth < excl + mine) {
+          uint32_t left = bits;
+          for (uint32_t i = excl; i < nth; ++i) left &= left - 1;
+          out_tokens[row] = static_cast<long long>(c0 + lane) * 8 - head + __ffs(left) - 1;
+          out_logprobs[row] = lp;
+        }
+        at += __shfl_sync(0xffffffffu, incl, 31);
+        if (nth < at) break;
+      }
+      return;
     }
   };
 
@@ -659,7 +678,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       if (tid < 64) sh.group_cnt[tid] = 0;
       __syncthreads();
       const uint32_t lo = static_cast<uint32_t>(groups - 1 - g) * 64;
-      load_batch(batch, tid, chunks);
+      load_first(batch, 0, chunks);
       for_each(batch, 0, chunks, [&](uint32_t w) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -720,7 +739,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     };
 
     double kept = sh.mass[groups - 1];
-    const int k = greedy || rw.min_p > 1.0 ? 1 : row_k;  // the first candidate stays whatever min_p asks
+    const int k = greedy || rw.min_p > 1.0 ? 1 : sh.set_k;  // the first candidate stays whatever min_p asks
     if (k > 0 && static_cast<uint32_t>(k) < n_all) {
       const uint32_t uk = static_cast<uint32_t>(k);
 #pragma unroll
@@ -749,8 +768,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       kept = sh.cum;
       __syncthreads();
     }
-    const double p = row_p;
-    const double uu = fmin(fmax(static_cast<double>(row_u), 0.0), 1.0 - 0x1p-53);  // NaN: 0
+    const double p = sh.set_p;
+    const double uu = fmin(fmax(static_cast<double>(sh.set_u), 0.0), 1.0 - 0x1p-53);  // NaN: 0
     // the cut by top-p, then the draw (a loop: one copy of the search's code)
 #pragma unroll 1
     for (int stage = p < 1.0 && !greedy ? 1 : 2; stage <= 2; ++stage) {
