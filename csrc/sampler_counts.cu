@@ -841,13 +841,17 @@ template <typename T>
 int sample_counts(const void* logits, long long ld, int rows, int V, const float* u, const float* temperature,
                   const int* top_k, const float* top_p, const float* min_p, long long* tokens, float* logprobs,
                   cudaStream_t s) {
-  // Few rows: spread each over more SMs while its slices stay long enough to count. Measured on V = 151936 (bf16, us
-  // by cluster size 1, 2, 4, 8): 1 row 38, 27, 20, 16; 64 rows 52, 35, 30, 46; 150 rows 65, 57, 62, 98; 256 rows 72,
-  // 74, 93, 156. Blocks of 1024 threads, one an SM, are what fp16's counters leave room for (bf16: 79 for 256 rows).
+  // Few rows: spread each over more SMs while its slices stay long enough to count and the GPU has room for them all at
+  // once: pairs as far as blocks fit, larger clusters on nine tenths of the SMs (they do not fill a GPC), one block
+  // each. Measured by cluster size 1, 2, 4, 8 in us: bf16, V = 151936: 1 row 28, 21, 17, 15; 30 rows 36, 26, 21, 22;
+  // 60 rows 35, 26, 26, 40; 130 rows 38, 35, 47, 79; 200 rows 56, 53, 68, 116; 256 rows 57, 64, 85, 146. V = 32000:
+  // 30 rows 19, 15, 14, 19; 74 rows 19, 16, 27, 46; 150 rows 24, 31, 43, 80. fp16, V = 151936: 18 rows 43, 32, 26, 44;
+  // 74 rows 45, 34, 69, 110. Blocks of 1024 threads, one an SM, are what fp16's counters leave room for.
   constexpr int threads = Key16<T>::kOneRow ? 1024 : 512;
-  const long long resident = static_cast<long long>(device_sm_count()) * (1024 / threads) * 21 / 20;
+  const long long sms = device_sm_count();
   int csize = 1;
-  while (csize < kCntMaxCluster && static_cast<long long>(rows) * csize * 2 <= resident && V / csize > 4096) csize *= 2;
+  for (int c = 2; c <= kCntMaxCluster && V / (c / 2) > 4096; c *= 2)
+    if (static_cast<long long>(rows) * c <= (c == 2 ? sms * (1024 / threads) : sms * 9 / 10)) csize = c;
   if (static_cast<long long>(rows) * csize > 0x7fffffffll) return -3;
   return launch_sample_counts<T, threads>(logits, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens, logprobs, csize, s);
 }
