@@ -239,7 +239,9 @@ struct RowPart {
 
 // One row per 2^lg threads, held in registers between the maximum and the rounding so that it is read once. PRE
 // turns the input row into the row to round: RMSNorm (x [rows, K], weight w) or SwiGLU (x = gate | up, [rows, 2K]),
-// with the roundings of the framework's own kernels (both give rows in T). For few rows: one wave of blocks.
+// with the roundings of the framework's own kernels (both give rows in T). Bound by memory where there are many rows
+// (bf16 [8192, 8960]: 43 us, 5.1 TB/s; RMSNorm, which reduces twice, 83 us; [2048, 4096]: 6.5 and 9.2 us, SwiGLU 11),
+// by one load, one or two reductions and one store in a row where there are few ([64, 1536]: 2.0, 2.6 and 2.4 us).
 template <typename T, int PRE, int NC>
 __global__ void __launch_bounds__(512) quantize_rows_kernel(const T* __restrict__ x, long long ldx,
                                                             const T* __restrict__ w, float eps,
@@ -378,8 +380,9 @@ __global__ void __launch_bounds__(kBulkThreads) quantize_rows_bulk_kernel(const 
   }
 }
 
-// Any K, stride and alignment: one block per row, element by element, the row read twice (the second time
-// from cache). For rows longer than the registers of a block hold, and for odd ones.
+// Any K, stride and alignment: one block per row, the row read twice (the second time from cache) in the aligned
+// chunks of 8 that cover it. For rows longer than the registers of a block hold, and for odd ones. Bound by
+// instructions: [4096, 4095] takes 21 us, where [4096, 4096] above takes 10 (element by element: 45).
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const T* __restrict__ x, long long ldx,
                                                                 int8_t* __restrict__ q, float* __restrict__ scale,
@@ -388,15 +391,53 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const T* __restr
   __shared__ uint32_t red_u[32];
   const long long row = blockIdx.x;
   const unsigned short* xr = reinterpret_cast<const unsigned short*>(x) + row * ldx;
-  uint32_t m = 0;
-  for (int c = threadIdx.x; c < K; c += blockDim.x) m = max(m, xr[c] & 0x7fffu);
-  const uint32_t amax = row_reduce(m, 8, red_u, [](uint32_t a, uint32_t b) { return max(a, b); });
+  // chunks of 8 elements from the 16-byte boundary at or before the row; zeros outside the row
+  const int head = static_cast<int>((reinterpret_cast<uintptr_t>(xr) & 15) >> 1);
+  const uint4* src = reinterpret_cast<const uint4*>(xr - head);
+  auto chunk = [&](int ch) -> uint4 {
+    const int i0 = ch * 8 - head;
+    if (i0 >= 0 && i0 + 8 <= K) return src[ch];
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = i0 + 2 * j, o = e + 1;
+      const uint32_t lo = (e >= 0 && e < K) ? xr[e] : 0u, hi = (o >= 0 && o < K) ? xr[o] : 0u;
+      w[j] = lo | (hi << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  uint32_t m2 = 0;
+  for (int c = threadIdx.x; c * 8 < head + K; c += blockDim.x) {
+    const uint4 v = chunk(c);
+    m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+  }
+  const uint32_t amax = row_reduce(amax_pair(m2), 8, red_u, [](uint32_t a, uint32_t b) { return max(a, b); });
   const RowQuant s = row_quant<T>(amax);
   if (threadIdx.x == 0) scale[row] = row_scale<T>(amax);
   const bool finite = amax < Half16<T>::kInf;
-  for (int c = threadIdx.x; c < Kp; c += blockDim.x)
-    q[row * Kp + c] = static_cast<int8_t>(
-        (c < K && finite) ? static_cast<int>(quant_bits(Half16<T>::one(xr[c]), s) & 0xffu) : 0);
+  for (int c = threadIdx.x; c * 8 < Kp; c += blockDim.x) {
+    // 8 elements of the row out of two chunks: a shift by `head` halves, the same for all of the row
+    const uint4 a = chunk(c), b = head ? chunk(c + 1) : make_uint4(0, 0, 0, 0);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (head & 4)
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    if (head & 2)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    if (head & 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Half16<T>::unpack(w[i]);
+      o[2 * i] = quant_bits(f.x, s);
+      o[2 * i + 1] = quant_bits(f.y, s);
+    }
+    *reinterpret_cast<uint2*>(q + row * Kp + c * 8) =
+        finite ? make_uint2(pack4(o[0], o[1], o[2], o[3]), pack4(o[4], o[5], o[6], o[7])) : make_uint2(0, 0);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -513,6 +554,9 @@ ACCERL_DEVINL void finish4(const Int8Params& p, long long t, int n, int4 acc, fl
 //   warp 0: TMA producer into a ring of stages;  warp 1: TMEM and MMA issue;  warps 2-5: accumulator to
 //   shared memory;  then all warps: a token row each, four neighbouring channels a lane (VEC: aligned rows) or
 //   every 32nd channel.
+// Bound by the latency of one CTA's chain (setup, first tile, exchange, store: about 4 us) where there are few tiles,
+// by memory where there are many. Measured without the quantising kernel: 1 x 1536 x 2048 4.9 us, 64 x 1536 x 17920
+// 11.5 us (2.6 TB/s), 256 x 8960 x 1536 14 us, 1 x 1536 x 151936 41 us (5.7 TB/s).
 template <int OUT, bool VEC>
 __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                       const __grid_constant__ CUtensorMap tmX,
@@ -802,6 +846,9 @@ ACCERL_DEVINL void add_residual32(float (&f)[32], const Int8Params& p, long long
 // tokens. Accumulators are double-buffered in TMEM, so the epilogue of a tile runs under the next one's
 // products. TMA_OUT: the result leaves through swizzled shared memory and TMA stores (16-byte aligned rows);
 // otherwise, and for residuals that are not aligned, through fp32 staging and coalesced element stores.
+// Bound by the tensor cores under the power cap and by what L2 delivers to them (0.33 us per 128 of K and tile: 5
+// stages of 32 KB a CTA keep them fed), and by the last wave. Measured without the quantising kernel: 8192 x 1536 x
+// 17920 179 us (2.5 POP/s), 8192 x 8960 x 1536 80 us (2.8), 2048 x 4096 x 24576 143 us (2.9); 8-bit dense peak 3.3.
 template <int OUT, bool TMA_OUT>
 __global__ void __launch_bounds__(kI8PairThreads, 1)
     gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -1126,12 +1173,16 @@ int launch_stream(const CUtensorMap& mw, const CUtensorMap& mx, const Int8Params
   return static_cast<int>(cudaLaunchKernelEx(&cfg, gemm_int8_stream_kernel<OUT, VEC>, mw, mx, p));
 }
 
+// SMs that clusters of `splits` CTAs can use at once, one CTA each: larger ones do not fill a GPC.
+int int8_room(int splits, int sms) { return splits >= 4 ? sms * 9 / 10 : sms; }
+
 // Which kernel runs a product: bt = 0 the persistent pairs, else the streaming kernel with bt tokens per tile and
 // `splits` CTAs per tile. The candidate with the least estimated cost wins. An estimate has a fixed part, a part per
 // 128 elements of K and one per token of the tile, times the share of an SM that a CTA gets (pairs: the waves); its
-// constants are fitted to the times of all candidates over M 1..4096 and eleven (K, N) from (300, 700) to (12288,
-// 4096) so that the choice is right (they are no times): the chosen candidate took 3 % longer than the best on
-// average. `store_ok`: TMA can store the result (element stores cost the pairs another 6 us a wave at N = 1111).
+// constants are fitted to the times of all candidates over M 1..4096 and fourteen (K, N) from (300, 700) to (1536,
+// 151936) so that the choice is right (they are no times): the chosen candidate took 1.4 % longer than the best on
+// average, 18 % at most. `store_ok`: TMA can store the result (element stores cost the pairs another 6 us a wave at
+// N = 1111).
 struct Int8Plan {
   int bt, splits;
 };
@@ -1139,7 +1190,7 @@ Int8Plan plan_int8(int M, int N, int K, bool store_ok, int sms) {
   const int kbs = (K + kI8BK - 1) / kI8BK;
   const double pair_tiles = static_cast<double>((M + kI8Tile - 1) / kI8Tile) * ((N + kI8Tile - 1) / kI8Tile);
   const double waves = std::ceil(pair_tiles / (sms / 2));
-  double best = 11.5 + waves * kbs * 0.343 + (waves - 1) * 0.67 + (store_ok ? 0.0 : waves * 6.0);
+  double best = 8.5 + waves * kbs * 0.326 + (waves - 1) * 2.06 + (store_ok ? 0.0 : waves * 6.0);
   Int8Plan plan{0, 1};
   for (int bt = 16; bt <= kI8MaxTokens && (bt == 16 || bt < 2 * M); bt *= 2) {
     if ((M + bt - 1) / bt > 65535) continue;  // a grid's second dimension
@@ -1147,9 +1198,10 @@ Int8Plan plan_int8(int M, int N, int K, bool store_ok, int sms) {
     for (int sp = 1; sp <= 8 && sp <= kbs; sp *= 2) {
       const double ctas = tiles * sp;
       if (sp > 1 && ctas > 4 * sms) break;
-      const double t = 3.5 + (sp > 1 ? 0.6 : 0.0) +
-                       (ctas > sms ? 1.515 * ctas / sms : 1.0) *
-                           (((kbs + sp - 1) / sp) * (0.179 + 0.00148 * bt) + 0.0272 * bt);
+      const double room = int8_room(sp, sms);
+      const double t = 6.47 + (sp > 1 ? 0.33 : 0.0) +
+                       (ctas <= room ? 1.0 : (ctas > 2 * room && sp == 1 ? 0.758 : 1.24) * ctas / room) *
+                           (((kbs + sp - 1) / sp) * (0.252 + 0.00177 * bt) + (sp > 1 ? 0.0197 : 0.0139) * bt);
       if (t < best) {
         best = t;
         plan = Int8Plan{bt, sp};
@@ -1304,8 +1356,11 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   const int stage_bytes = (kI8Rows + p.bt) * kI8BK;
   // the accumulator: behind the stages where peers write it, else where the stages were
   const int acc_bytes = p.bt * kI8Rows * 4;
-  const bool alone = static_cast<long long>(grid.x) * grid.y * grid.z <= device_sm_count();  // on its SM
-  const int room = (alone ? 200 : 100) * 1024 - (plan.splits > 1 ? acc_bytes : 0);
+  // One CTA on an SM gets all of its shared memory, two half each. Of more, three an SM: while one finishes its tile the
+  // others load (the LM head, 1 x 1536 x 151936: 46 us with two an SM, 41 with three, 43 with four).
+  const long long ctas = static_cast<long long>(grid.x) * grid.y * grid.z, sms = int8_room(plan.splits, device_sm_count());
+  const int room = (ctas <= sms ? 200 : (ctas > 2 * sms && plan.splits == 1 ? 72 : 100)) * 1024 -
+                   (plan.splits > 1 ? acc_bytes : 0);
   p.stages = std::max(2, std::min({16, (kbs + plan.splits - 1) / plan.splits, room / stage_bytes}));
   const int smem_bytes =
       (plan.splits > 1 ? p.stages * stage_bytes + acc_bytes : std::max(p.stages * stage_bytes, acc_bytes)) + 1024;

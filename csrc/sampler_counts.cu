@@ -241,7 +241,12 @@ struct RowWeights {
   ACCERL_DEVINL bool kept(uint32_t key, double w) const { return key == max_key || !(min_p > 0.0) || w >= min_p; }
 };
 
-// One row per cluster of CTAs, each counting a slice of it.
+// One row per cluster of CTAs, each counting a slice of it. Two passes over the row, the second for half of it on
+// average and from L2; between them nothing depends on V. Measured (bf16, V = 151936): 256 rows 52 us, of which the
+// reads need 12: shared memory adds up 32 counters at random banks in 3 to 4 clocks, so two rows on an SM, counted one
+// behind the other, take 27 us, the sums over the groups and the searches 15, the token's place 5. 1 row in 15 us, nearly
+// all of it latency (barriers of the cluster, sums of 64-bit floats, dependent searches). fp16's wider range of
+// values in use means 350 pairs of groups: 100 rows of 32003 take 26 us, 11 of them there.
 template <typename T, int kCntThreads>
 __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     sample_counts_kernel(const T* __restrict__ logits, long long ld, int V, const float* __restrict__ u,
