@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       return bits;
     };
     // The CTA counts strip after strip until one holds the token, each warp a contiguous part; the warp that has it
-    // goes through its part again. (256 rows of 151936: half of the row on average, 9 us of them for 13.)
+    // goes through its part again. (256 rows of 151936: half of the row on average, 5 us for 13.)
     constexpr int kBatch = 8;
     const int wper = min(32 * kBatch, (b - a + kCntWarps - 1) / kCntWarps);
     uint32_t base = 0;

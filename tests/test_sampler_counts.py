@@ -130,6 +130,35 @@ def test_large_vocabularies(rows, v):
     assert torch.equal(tok1.cpu(), etok1)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,v", [(160, 40001), (90, 140003), (5, 300007)])
+@pytest.mark.parametrize("value", [0.5, -3.0, 0.0, 1000.0, 1e-13])
+def test_every_place_of_long_rows(dtype, rows, v, value):
+    """Rows of one value: the draw's number alone names the token, in every part of rows that start at any alignment
+    (fp16 1000 and bf16 1e-13 lie outside the counters' window; fp16 rounds 1e-13 to zero)."""
+    x = torch.full((rows, v), value, dtype=torch.float64).to(dtype).cuda()
+    u = ((torch.arange(rows) + 0.5) / rows).float()
+    u[0], u[-1] = 0.0, 1.0 - 2.0 ** -24
+    tok, lp = ops.sample_inverse_cdf(x, u.cuda(), full(rows, 1.0, "cuda"))
+    assert tok.tolist() == [int(float(n) * v) for n in u]  # a product below 2^53 of 24 and 19 bits: exact
+    torch.testing.assert_close(lp.cpu(), full(rows, -math.log(v), "cpu"), rtol=2.0 ** -23, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,v", [(150, 40001), (80, 70003)])
+def test_many_long_rows(dtype, rows, v):
+    x, u, _ = make(rows, v, "cuda", dtype, seed=rows)
+    t, p, k = full(rows, 0.9, "cuda"), full(rows, 0.97, "cuda"), full(rows, 500, "cuda", torch.int32)
+    for kk, pp in ((None, None), (k, None), (None, p), (k, p)):
+        tok, lp = ops.sample_inverse_cdf(x, u, t, top_k=kk, top_p=pp)
+        etok, elp = ops.sample_inverse_cdf(x.cpu(), u.cpu(), t.cpu(), top_k=kk.cpu() if kk is not None else None,
+                                           top_p=pp.cpu() if pp is not None else None)
+        assert torch.equal(tok.cpu(), etok)
+        torch.testing.assert_close(lp.cpu(), elp, rtol=2.0 ** -23, atol=1e-12)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_ties_go_to_the_lowest_index(device, dtype):
