@@ -140,10 +140,25 @@ def profile_case(kind: str):
     * ``opsprof``: RMSNorm fwd/bwd, RoPE, SwiGLU fwd/bwd, embedding fwd/bwd, log-softmax/label
       fwd/bwd on 4096 response rows of a 151936 vocabulary, policy loss, AdamW on 64 M parameters;
     * ``decodeprof``: paged decode attention for 256 sequences of 1024 cached tokens, KV-cache write
-      and sampling of 256 rows of a 151936 vocabulary.
+      and sampling of 256 rows of a 151936 vocabulary;
+    * ``int8prof``: 8-bit linear layers (gate_up of 8192 and 64 tokens, LM head of one token, both of the 1.5B
+      shape), SwiGLU rows to 8 bits, sampling of 256 rows of a 151936 vocabulary by counting.
     """
     dev = "cuda"
-    if kind == "attnprof":
+    if kind == "int8prof":
+        w = ops.quantize_rows((torch.randn(17920, 1536, device=dev) * 0.02).bfloat16())
+        head = ops.quantize_rows((torch.randn(151936, 1536, device=dev) * 0.02).bfloat16())
+        x = torch.randn(8192, 1536, device=dev).bfloat16()
+        gu = torch.randn(8192, 2 * 8960, device=dev).bfloat16()
+        logits = (torch.randn(256, 151936, device=dev) * 2).bfloat16()
+        u = torch.rand(256, device=dev)
+        temp, top_p = torch.full((256,), 0.8, device=dev), torch.full((256,), 0.95, device=dev)
+        ops.sample_inverse_cdf(logits, u, temp, top_p=top_p)
+        ops.linear_int8(x, w)
+        ops.linear_int8(x[:64], w)
+        ops.linear_int8(x[:1], head)
+        ops.swiglu_quantize(gu)
+    elif kind == "attnprof":
         Hq, Hkv, D, T = 12, 2, 128, 4096
         cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
         qkv = torch.randn(T, (Hq + 2 * Hkv) * D, device=dev).bfloat16()
@@ -277,7 +292,7 @@ def bench_int8(results):
         t8 = median_ms(lambda: ops.linear_int8(x, w8))
         t16 = median_ms(lambda: ops.linear(x, w))
         flops, nbytes = 2.0 * M * N * K, 2 * M * K + N * K + 2 * M * N
-        results[f"int8/{M}x{K}x{N}"] = {"ms": t8, "tflops": flops / t8 / 1e9, "gbs": nbytes / t8 / 1e6, "bf16_ms": t16,
+        results[f"int8/{M}x{K}x{N}"] = {"ms": t8, "tops": flops / t8 / 1e9, "gbs": nbytes / t8 / 1e6, "bf16_ms": t16,
                                         "floor_ms": max(flops / (2 * peak_tf) / 1e9, nbytes / peak_gbs / 1e6)}
         del x, w, w8
     for rows, V in ((1, 151936), (64, 151936), (256, 151936)):
@@ -289,7 +304,7 @@ def bench_int8(results):
                                                      "frac_hbm": 2 * rows * V / t / 1e6 / peak_gbs}
 
 
-PROFILE_CASES = ("attnprof", "gemmprof", "moeprof", "opsprof", "decodeprof")
+PROFILE_CASES = ("attnprof", "gemmprof", "moeprof", "opsprof", "decodeprof", "int8prof")
 
 
 def main():
