@@ -2,6 +2,7 @@
 // expose extern "C" launchers; this file validates tensors and forwards raw pointers together with
 // the current CUDA stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
@@ -813,20 +814,24 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
 // C++ runtime is not the one torch was built with.
 std::string num(int64_t v) { return std::to_string(v); }
 
-// x [rows, K] (pre 0: as it is, 1: RMSNorm with weight w, 2: SwiGLU of gate | up [rows, 2K]) -> int8 rows
-// q [rows, K rounded up to 16] and scale [rows], allocated when not given.
-std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w,
-                                                 double eps, const c10::optional<at::Tensor>& q_out,
-                                                 const c10::optional<at::Tensor>& scale_out, const at::Tensor& status) {
+// A tensor on the current CUDA device, without the dispatcher's way (a microsecond of a call of ten).
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef size, at::ScalarType type) {
+  return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);
+}
+
+struct RowsToQuantize {
+  int64_t rows, K, Kp;
+};
+// Refuses what accerl_quantize_rows does not take (pre 0: x [rows, K] as it is, 1: RMSNorm with weight w, 2: SwiGLU of
+// gate | up [rows, 2K]).
+RowsToQuantize check_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be [rows, features]");
-  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
-  const bool half = x.scalar_type() == at::kHalf;
-  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || (half && pre == 0), 
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || (x.scalar_type() == at::kHalf && pre == 0),
                     std::string("x must be bfloat16") + (pre == 0 ? " or float16" : "") + ", got " +
                         c10::toString(x.scalar_type()));
   TORCH_CHECK_VALUE(x.stride(1) == 1 || x.size(1) == 1, "the last dimension of x must be contiguous");
   TORCH_CHECK_VALUE(pre != 2 || x.size(1) % 2 == 0, "gate | up must be [rows, 2K]");
-  const int64_t rows = x.size(0), K = pre == 2 ? x.size(1) / 2 : x.size(1), Kp = (K + 15) / 16 * 16;
+  const int64_t rows = x.size(0), K = pre == 2 ? x.size(1) / 2 : x.size(1);
   TORCH_CHECK_VALUE(rows <= 0x7fffffff && K < 0x7fffff00, "too many rows or features");
   if (pre != 0) {
     const bool aligned = K % 8 == 0 && K <= 32768 && (rows <= 1 || x.stride(0) % 8 == 0) &&
@@ -838,24 +843,37 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pr
                           w->scalar_type() == at::kBFloat16 && reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0,
                       "the norm weight must be contiguous bfloat16 [" + num(K) + "] on x's device, aligned to 16 bytes");
   }
+  return {rows, K, (K + 15) / 16 * 16};
+}
+void launch_quantize(const at::Tensor& x, const RowsToQuantize& r, int64_t pre, const c10::optional<at::Tensor>& w,
+                     double eps, void* q, float* scale, const at::Tensor& status) {
+  check(accerl_quantize_rows(x.data_ptr(), r.rows <= 1 ? 0 : x.stride(0), x.scalar_type() == at::kHalf,
+                             static_cast<int>(pre), opt_ptr(w), static_cast<float>(eps), q, scale, r.rows,
+                             static_cast<int>(r.K), status.data_ptr<int>(), cur_stream()),
+        "quantize_rows");
+}
+
+// x -> int8 rows q [rows, K rounded up to 16] and scale [rows], allocated when not given.
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, int64_t pre, const c10::optional<at::Tensor>& w,
+                                                 double eps, const c10::optional<at::Tensor>& q_out,
+                                                 const c10::optional<at::Tensor>& scale_out, const at::Tensor& status) {
+  const RowsToQuantize r = check_rows(x, pre, w);
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
   at::Tensor q, scale;
   if (q_out.has_value()) {
     q = *q_out;
     scale = *scale_out;
-    TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.is_contiguous() && q.dim() == 2 && q.size(0) == rows &&
-                          q.size(1) == Kp && scale.scalar_type() == at::kFloat && scale.is_contiguous() &&
-                          scale.numel() == rows && q.device() == x.device() && scale.device() == x.device() &&
+    TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.is_contiguous() && q.dim() == 2 && q.size(0) == r.rows &&
+                          q.size(1) == r.Kp && scale.scalar_type() == at::kFloat && scale.is_contiguous() &&
+                          scale.numel() == r.rows && q.device() == x.device() && scale.device() == x.device() &&
                           reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
-                      "out does not hold " + num(rows) + " x " + num(K) + " int8 rows on " + x.device().str() +
+                      "out does not hold " + num(r.rows) + " x " + num(r.K) + " int8 rows on " + x.device().str() +
                           ", aligned to 16 bytes");
   } else {
-    q = at::empty({rows, Kp}, x.options().dtype(at::kChar));
-    scale = at::empty({rows}, x.options().dtype(at::kFloat));
+    q = empty_on(x, {r.rows, r.Kp}, at::kChar);
+    scale = empty_on(x, {r.rows}, at::kFloat);
   }
-  check(accerl_quantize_rows(x.data_ptr(), rows <= 1 ? 0 : x.stride(0), half, static_cast<int>(pre), opt_ptr(w),
-                             static_cast<float>(eps), q.data_ptr(), scale.data_ptr<float>(), rows, static_cast<int>(K),
-                             status.data_ptr<int>(), cur_stream()),
-        "quantize_rows");
+  launch_quantize(x, r, pre, w, eps, q.data_ptr(), scale.data_ptr<float>(), status);
   return {q, scale};
 }
 
@@ -864,37 +882,37 @@ int float_type_id(at::ScalarType t) {
   return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1;
 }
 
-// out [M, N] = sx sw (qx qw^T) (+ bias) (+ residual), out allocated when not given
-at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
-                     const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
-                     const c10::optional<at::Tensor>& out_opt, const c10::optional<at::ScalarType>& out_dtype,
-                     const at::Tensor& status, bool w_early) {
-  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(qw));
-  const int64_t M = qx.size(0), N = qw.size(0), Kp = (K + 15) / 16 * 16;
-  const auto dev = qw.device();
-  auto on_device = [&](const at::Tensor& t) {
-    TORCH_CHECK_VALUE(t.device() == dev, "every tensor must be on the weight's device " + dev.str() + ", got one on " + t.device().str());
-  };
-  on_device(qx), on_device(sx), on_device(sw);
+void check_device(const at::Tensor& t, const at::Tensor& weight) {
+  TORCH_CHECK_VALUE(t.device() == weight.device(), "every tensor must be on the weight's device " + weight.device().str() +
+                                                       ", got one on " + t.device().str());
+}
+void check_int8_rows(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& weight, int64_t K) {
   TORCH_CHECK_VALUE(K > 0 && K <= 133144, "in must be at most 133144, got " + num(K));
-  for (const at::Tensor* q : {&qx, &qw})
-    TORCH_CHECK_VALUE(q->scalar_type() == at::kChar && q->dim() == 2 && q->is_contiguous() && q->size(1) == Kp &&
-                          reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 == 0,
-                      "int8 rows must be contiguous [rows, in rounded up to 16], aligned to 16 bytes");
-  TORCH_CHECK_VALUE(sx.scalar_type() == at::kFloat && sw.scalar_type() == at::kFloat && sx.is_contiguous() &&
-                        sw.is_contiguous() && sx.numel() == M && sw.numel() == N,
+  check_device(scale, weight);
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && q.dim() == 2 && q.is_contiguous() && q.size(1) == (K + 15) / 16 * 16 &&
+                        reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+                    "int8 rows must be contiguous [rows, in rounded up to 16], aligned to 16 bytes");
+  TORCH_CHECK_VALUE(scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.numel() == q.size(0),
                     "int8 rows must have one contiguous float32 scale each");
-  TORCH_CHECK_VALUE(M <= 0x3fffffff && N <= 0x3fffffff, "too many rows");
+  TORCH_CHECK_VALUE(q.size(0) <= 0x3fffffff, "too many rows");
+}
+
+// out [M, N] = sx sw (qx qw^T) (+ bias) (+ residual), out allocated when not given; qx and sx have been checked
+at::Tensor product_int8(const void* qx, const float* sx, int64_t M, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
+                        const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                        const c10::optional<at::Tensor>& out_opt, const c10::optional<at::ScalarType>& out_dtype,
+                        const at::Tensor& status, bool w_early) {
+  const int64_t N = qw.size(0);
   at::Tensor out;
   if (out_opt.has_value()) {
     out = *out_opt;
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == M && out.size(1) == N && float_type_id(out.scalar_type()) >= 0 &&
                           (N <= 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N),
                       "out must be bf16, fp16 or fp32 [" + num(M) + ", " + num(N) + "] with a contiguous last dimension");
-    on_device(out);
+    check_device(out, qw);
   } else {
     TORCH_CHECK_VALUE(out_dtype.has_value() && float_type_id(*out_dtype) >= 0, "out_dtype must be bf16, fp16 or fp32");
-    out = at::empty({M, N}, qw.options().dtype(*out_dtype));
+    out = empty_on(qw, {M, N}, *out_dtype);
   }
   int in_type = float_type_id(out.scalar_type());
   long long ldr = 0;
@@ -902,7 +920,7 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
     TORCH_CHECK_VALUE(residual->dim() == 2 && residual->size(0) == M && residual->size(1) == N &&
                           float_type_id(residual->scalar_type()) >= 0 && (N <= 1 || residual->stride(1) == 1),
                       "residual must be bf16, fp16 or fp32 [" + num(M) + ", " + num(N) + "] with a contiguous last dimension");
-    on_device(*residual);
+    check_device(*residual, qw);
     in_type = float_type_id(residual->scalar_type());
     ldr = residual->stride(0);
   }
@@ -910,17 +928,29 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->numel() == N && bias->is_contiguous() &&
                           float_type_id(bias->scalar_type()) >= 0,
                       "bias must be contiguous bf16, fp16 or fp32 [" + num(N) + "]");
-    on_device(*bias);
+    check_device(*bias, qw);
     TORCH_CHECK_VALUE(!residual.has_value() || bias->scalar_type() == residual->scalar_type(),
                       "bias and residual must be of one type");
     in_type = float_type_id(bias->scalar_type());
   }
-  check(accerl_gemm_int8(qx.data_ptr(), sx.data_ptr<float>(), qw.data_ptr(), sw.data_ptr<float>(),
+  check(accerl_gemm_int8(qx, sx, qw.data_ptr(), sw.data_ptr<float>(),
                          static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), opt_ptr(bias),
                          opt_ptr(residual), ldr, in_type, out.data_ptr(), M <= 1 ? N : out.stride(0),
                          float_type_id(out.scalar_type()), w_early, status.data_ptr<int>(), cur_stream()),
         "gemm_int8");
   return out;
+}
+
+at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
+                     const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                     const c10::optional<at::Tensor>& out, const c10::optional<at::ScalarType>& out_dtype,
+                     const at::Tensor& status, bool w_early) {
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(qw));
+  check_device(qx, qw), check_device(sx, qw);
+  check_int8_rows(qw, sw, qw, K);
+  check_int8_rows(qx, sx, qw, K);
+  return product_int8(qx.data_ptr(), sx.data_ptr<float>(), qx.size(0), qw, sw, K, bias, residual, out, out_dtype, status,
+                      w_early);
 }
 
 // The same from bf16 / fp16 activations: quantised first, the product launched to start behind that kernel.
@@ -929,11 +959,18 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& qw, const at::Tens
                        const c10::optional<at::Tensor>& out, const c10::optional<at::ScalarType>& out_dtype,
                        const at::Tensor& status) {
   TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "inner dimensions differ (x needs " + num(K) + " columns)");
-  TORCH_CHECK_VALUE(x.device() == qw.device(), "every tensor must be on the weight's device " + qw.device().str() + ", got one on " + x.device().str());
-  auto [qx, sx] = quantize_rows(x, 0, c10::nullopt, 0.0, c10::nullopt, c10::nullopt, status);
-  if (g_last_rc != 0) return qx;  // reported by the caller
-  return gemm_int8(qx, sx, qw, sw, K, bias, residual, out, out_dtype.has_value() ? out_dtype : x.scalar_type(), status,
-                   true);
+  check_device(x, qw);
+  const RowsToQuantize r = check_rows(x, 0, c10::nullopt);
+  check_int8_rows(qw, sw, qw, K);
+  const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(x));
+  const int64_t q_bytes = r.rows * r.Kp;  // a multiple of 16; the scales follow
+  const at::Tensor ws = empty_on(x, {q_bytes + r.rows * 4}, at::kChar);
+  char* q = static_cast<char*>(ws.data_ptr());
+  float* scale = reinterpret_cast<float*>(q + q_bytes);
+  launch_quantize(x, r, 0, c10::nullopt, 0.0, q, scale, status);
+  if (g_last_rc != 0) return ws;  // reported by the caller
+  return product_int8(q, scale, r.rows, qw, sw, K, bias, residual, out, out_dtype.has_value() ? out_dtype : x.scalar_type(),
+                      status, true);
 }
 
 }  // namespace
