@@ -846,8 +846,9 @@ ACCERL_DEVINL void add_residual32(float (&f)[32], const Int8Params& p, long long
 // tokens. Accumulators are double-buffered in TMEM, so the epilogue of a tile runs under the next one's
 // products. TMA_OUT: the result leaves through swizzled shared memory and TMA stores (16-byte aligned rows);
 // otherwise, and for residuals that are not aligned, through fp32 staging and coalesced element stores.
-// Bound by the tensor cores under the power cap and by what L2 delivers to them (0.33 us per 128 of K and tile: 5
-// stages of 32 KB a CTA keep them fed), and by the last wave. Measured without the quantising kernel: 8192 x 1536 x
+// Bound by what L2 delivers (64 KB per 128 of K and tile: 12 to 14 TB/s in all; 5 stages, 4 cost 3 % more), where K is
+// short also by the result's way through it (8192 x 1536 x 17920: 152 us without an epilogue, 157 without its stores),
+// and by the last wave. Measured without the quantising kernel: 8192 x 1536 x
 // 17920 179 us (2.5 POP/s), 8192 x 8960 x 1536 80 us (2.8), 2048 x 4096 x 24576 143 us (2.9); 8-bit dense peak 3.3.
 template <int OUT, bool TMA_OUT>
 __global__ void __launch_bounds__(kI8PairThreads, 1)
