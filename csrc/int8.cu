@@ -1182,16 +1182,17 @@ int int8_room(int splits, int sms) { return splits >= 4 ? sms * 9 / 10 : sms; }
 // 128 elements of K and one per token of the tile, times the share of an SM that a CTA gets (pairs: the waves); its
 // constants are fitted to the times of all candidates over M 1..4096 and fourteen (K, N) from (300, 700) to (1536,
 // 151936) so that the choice is right (they are no times): the chosen candidate took 1.4 % longer than the best on
-// average, 18 % at most. `store_ok`: TMA can store the result (element stores cost the pairs another 6 us a wave at
-// N = 1111).
+// average, 18 % at most. `store_ok`: TMA can store the result; `vec`: the streaming kernel can store four channels at
+// once. What element stores cost either is fitted to eight more (K, N) with such N (512 x 17913 to 8000 x 1537): 3 %
+// longer on average, 31 % at most (without: 5 % and 113 %).
 struct Int8Plan {
   int bt, splits;
 };
-Int8Plan plan_int8(int M, int N, int K, bool store_ok, int sms) {
+Int8Plan plan_int8(int M, int N, int K, bool store_ok, bool vec, int sms) {
   const int kbs = (K + kI8BK - 1) / kI8BK;
   const double pair_tiles = static_cast<double>((M + kI8Tile - 1) / kI8Tile) * ((N + kI8Tile - 1) / kI8Tile);
   const double waves = std::ceil(pair_tiles / (sms / 2));
-  double best = 8.5 + waves * kbs * 0.326 + (waves - 1) * 2.06 + (store_ok ? 0.0 : waves * 6.0);
+  double best = 8.5 + waves * kbs * 0.326 + (waves - 1) * 2.06 + (store_ok ? 0.0 : 6.0 + waves * 10.0);
   Int8Plan plan{0, 1};
   for (int bt = 16; bt <= kI8MaxTokens && (bt == 16 || bt < 2 * M); bt *= 2) {
     if ((M + bt - 1) / bt > 65535) continue;  // a grid's second dimension
@@ -1202,7 +1203,8 @@ Int8Plan plan_int8(int M, int N, int K, bool store_ok, int sms) {
       const double room = int8_room(sp, sms);
       const double t = 6.47 + (sp > 1 ? 0.33 : 0.0) +
                        (ctas <= room ? 1.0 : (ctas > 2 * room && sp == 1 ? 0.758 : 1.24) * ctas / room) *
-                           (((kbs + sp - 1) / sp) * (0.252 + 0.00177 * bt) + (sp > 1 ? 0.0197 : 0.0139) * bt);
+                           (((kbs + sp - 1) / sp) * (0.252 + 0.00177 * bt) +
+                            ((sp > 1 ? 0.0197 : 0.0139) + (vec ? 0.0 : 0.02)) * bt);
       if (t < best) {
         best = t;
         plan = Int8Plan{bt, sp};
@@ -1331,7 +1333,10 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   const int es = out_type == kOutF32 ? 4 : 2, rs = in_type == kOutF32 ? 4 : 2;
   const bool store_ok = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo * es % 16 == 0 && ldo >= N &&
                         (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && ldr * rs % 16 == 0));
-  const Int8Plan plan = plan_int8(M, N, K, store_ok, device_sm_count());
+  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo % 4 == 0 &&
+                   (reinterpret_cast<uintptr_t>(sw) & 15) == 0 &&
+                   (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && ldr % 4 == 0));
+  const Int8Plan plan = plan_int8(M, N, K, store_ok, vec, device_sm_count());
   CUtensorMap mx, mw, mo;
   if (plan.bt == 0) {
     p.tiles_m = (M + kI8Tile - 1) / kI8Tile;
@@ -1367,9 +1372,6 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
       (plan.splits > 1 ? p.stages * stage_bytes + acc_bytes : std::max(p.stages * stage_bytes, acc_bytes)) + 1024;
   if (!make_int8_map(&mw, qw, Kp, static_cast<uint64_t>(N), kI8Rows)) return -7;
   if (!make_int8_map(&mx, qx, Kp, static_cast<uint64_t>(M), static_cast<uint32_t>(p.bt))) return -8;
-  const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo % 4 == 0 &&
-                   (reinterpret_cast<uintptr_t>(sw) & 15) == 0 &&
-                   (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && ldr % 4 == 0));
   auto launch = [&](auto type) {
     constexpr int OUT = decltype(type)::value;
     return vec ? launch_stream<OUT, true>(mw, mx, p, grid, smem_bytes, stream)
