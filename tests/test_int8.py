@@ -110,6 +110,19 @@ def test_quantize_rows_extremes(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k,stride", [(1, 5), (6, 6), (9, 20), (257, 263), (1001, 1001), (2056, 2063), (4100, 4111)])
+def test_quantize_rows_at_every_alignment(device, dtype, k, stride):
+    """Rows that start anywhere between 16-byte boundaries, NaN all around them."""
+    rows = 11
+    for first in range(9):
+        flat = torch.full((first + rows * stride + 8,), float("nan"), dtype=dtype, device=device)
+        x = flat.as_strided((rows, k), (stride, 1), first)
+        x.copy_(randn(rows, k, seed=first, device=device, dtype=dtype))
+        check_rows(x, ops.quantize_rows(x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_quantize_rows_strides_and_out(device):
     base = randn(12, 200, device=device)
     for x in (base[:, 8:72], base[:, 3:80], base[::2, :64], base[2:3].expand(4, -1), base[:, :1]):
