@@ -40,6 +40,7 @@ struct Key16<__nv_bfloat16> {
   static constexpr uint32_t kBase = (127u - 40u) << 7, kSlots = 64u << 7, kMantissa = 7;
   static constexpr bool kOneRow = false;  // the counters leave room for two blocks on an SM
   static ACCERL_DEVINL float value(uint32_t bits) { return __uint_as_float(bits << 16); }
+  static ACCERL_DEVINL uint32_t bits(float v) { return __float_as_uint(v) >> 16; }  // of a neighbour: cut off
   static ACCERL_DEVINL uint32_t max2(uint32_t a, uint32_t b) {  // of both halves; a NaN loses
     const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
@@ -73,6 +74,7 @@ struct Key16<__half> {
   static ACCERL_DEVINL float value(uint32_t bits) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
   }
+  static ACCERL_DEVINL uint32_t bits(float v) { return __half_as_ushort(__float2half_rn(v)); }
   static ACCERL_DEVINL uint32_t max2(uint32_t a, uint32_t b) {
     const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
@@ -162,7 +164,7 @@ struct CountShared {
   uint32_t warp_u[3][32];
   double warp_d[32];
   double exp2_table[64];            // 2^(j / 64)
-  double ratio[2][64];              // of neighbouring values' masses by binade of the window: at T, at 1
+  double ratio[2][65];              // of neighbouring values' masses by binade of the window (and the padding): at T, at 1
   // of every CTA's slice: the largest key, whether a value lies below the window, whether one escapes it otherwise
   uint32_t max_key[kCntMaxCluster], any_low[kCntMaxCluster], escape[kCntMaxCluster];
   uint32_t group_cnt[64];                     // slow path: tokens of a group's values
@@ -200,9 +202,8 @@ constexpr double kLog2e64 = 64 * 1.44269504088896340736;
 template <typename T>
 struct RowWeights {
   double scale;  // 64 log2(e) / T
-  double min_p;
   float max;     // the row's largest logit
-  uint32_t max_key;
+  uint32_t max_key, keep_key;  // its key, and that of the smallest value that min_p keeps
   const double* table;
   ACCERL_DEVINL double gap(uint32_t key) const {
     return static_cast<double>(Key16<T>::value(key_bits(key))) - static_cast<double>(max);
@@ -238,7 +239,27 @@ struct RowWeights {
       for (int j = 0; j < 4; ++j) w[j] = key[j] > max_key ? 0.0 : mass(key[j], sc);
     }
   }
-  ACCERL_DEVINL bool kept(uint32_t key, double w) const { return key == max_key || !(min_p > 0.0) || w >= min_p; }
+  ACCERL_DEVINL bool kept(uint32_t key) const { return key >= keep_key; }
+  // The smallest key whose weight is at least min_p, by the whole warp: found once, so that every later question is one
+  // of whole numbers and has one answer. `lo` is not kept, `hi` is; all lanes but 0 try a key between them. The first
+  // try is around max + T log(min_p), which all but always holds the border; then the range shrinks by 32 a turn.
+  ACCERL_DEVINL uint32_t smallest_kept(float min_p, float t, int lane) const {
+    int lo = static_cast<int>(Key16<T>::kNegInf), hi = static_cast<int>(max_key), step = 1;
+    const float near = max + t * logf(fminf(min_p, 1.f));
+    const uint32_t near_bits = Key16<T>::bits(near);
+    int top = (near_bits & 0x7fffu) > Key16<T>::kInf ? hi : min(hi, static_cast<int>(bits_key(near_bits)) + 16);
+    while (hi - lo > 1) {
+      const int key = top - lane * step;
+      const uint32_t yes =
+          __ballot_sync(0xffffffffu, key >= hi || (key > lo && weight(static_cast<uint32_t>(key)) >= static_cast<double>(min_p)));
+      const int n = yes == 0xffffffffu ? 32 : __ffs(~yes) - 1;  // so many from the top are kept
+      if (n > 0) hi = min(hi, top - (n - 1) * step);
+      if (n < 32) lo = ::max(lo, top - n * step);
+      step = (hi - lo + 31) / 32;
+      top = hi;
+    }
+    return static_cast<uint32_t>(hi);
+  }
 };
 
 // One row per cluster of CTAs, each counting a slice of it. Two passes over the row, the second for half of it on
@@ -428,8 +449,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
   RowWeights<T> rw;
   rw.scale = kLog2e64 / td;
   rw.table = sh.exp2_table;
-  rw.min_p = row_min;
   rw.max_key = max_key;
+  rw.keep_key = 0u;  // min_p off
   rw.max = Key16<T>::value(key_bits(max_key));
   // what lies below the window is at most its lower edge
   const float edge = -Key16<T>::value(Key16<T>::kBase + S);
@@ -437,7 +458,22 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       !(static_cast<double>(rw.max) - static_cast<double>(edge) > kCntNegligible * fmax(td, 1.0));
   const bool slow = max_key != 0u && (escape != 0u || (any_low != 0u && low_matters));
   const bool empty = rw.max_key == 0u;
+  if (row_min > 0.f && !empty) rw.keep_key = rw.smallest_kept(row_min, static_cast<float>(td), lane);
 
+  // Keys of the four bins from b0 on, a multiple of 4, whose lowest is key0, and their weights at T and as exp(x - max).
+  // The sums over the groups and the searches inside one take a value's weight from here: a group that has mass for the
+  // one has it for the other.
+  auto quad_keys = [&](uint32_t b0, uint32_t key0, uint32_t (&key)[4]) -> bool {
+    // four neighbours, but in the group of zero, which has one value; the slow path's keys lie anywhere: no table
+    const uint32_t step = slow || b0 >= 64u ? 1u : 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) key[j] = key0 + j * step;
+    return !slow && step != 0u;
+  };
+  auto quad_weights = [&](const uint32_t (&key)[4], bool even, int plain, double (&w)[4]) {
+    const uint32_t binade = even ? ((key_bits(key[3]) & 0x7fffu) - Key16<T>::kBase) >> Key16<T>::kMantissa : 0u;
+    rw.mass4(key, even, sh.ratio[plain][binade], plain ? kLog2e64 : rw.scale, w);
+  };
   // Tokens and mass of the n groups of 64 bins in the counters, group i into the leader's arrays at order(i): four
   // bins a lane, half a warp a group, the groups spread over the cluster.
   double lse = 0.0;
@@ -464,17 +500,13 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
         // the leader's counters of these bins, which nobody else reads, take the whole cluster's counts
         if (csize > 1) *reinterpret_cast<uint4*>(peer(hist, 0) + b0) = make_uint4(c[0], c[1], c[2], c[3]);
         double w[4];
-        // four neighbours, but in the group of zero, which has one value
-        const uint32_t key0 = key_of(b0), step = slow || b0 >= 64u ? 1u : 0u;
-        const uint32_t key[4] = {key0, key0 + step, key0 + 2u * step, key0 + 3u * step};
-        // the slow path's keys lie anywhere: no table
-        const bool even = !slow && step != 0u;
-        const uint32_t binade = even ? ((key_bits(key[3]) & 0x7fffu) - Key16<T>::kBase) >> Key16<T>::kMantissa : 0u;
+        uint32_t key[4];
+        const bool even = quad_keys(b0, key_of(b0), key);
         auto take = [&](const double (&at_t)[4], const double (&at_1)[4]) {
           double mk[4], ml[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t k = rw.kept(key[j], at_t[j]) ? c[j] : 0u;
+            const uint32_t k = rw.kept(key[j]) ? c[j] : 0u;
             num += k;
             mk[j] = count_f64(k) * at_t[j];  // a weight is finite
             ml[j] = count_f64(c[j]) * at_1[j];
@@ -482,12 +514,12 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
           m = (mk[0] + mk[1]) + (mk[2] + mk[3]);
           lse += (ml[0] + ml[1]) + (ml[2] + ml[3]);
         };
-        rw.mass4(key, even, sh.ratio[0][binade], rw.scale, w);
+        quad_weights(key, even, 0, w);
         if (t == 1.f) {
           take(w, w);
         } else {  // the two chains of operations overlap
           double w1[4];
-          rw.mass4(key, even, sh.ratio[1][binade], kLog2e64, w1);
+          quad_weights(key, even, 1, w1);
           take(w, w1);
         }
 #pragma unroll
@@ -666,14 +698,16 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
         n[0] = sh.group_cnt[63 - 2 * lane];
         n[1] = sh.group_cnt[62 - 2 * lane];
       }
+      const uint32_t b0 = b & ~3u;
+      uint32_t k4[4];
+      double w4[4];
+      const bool even = quad_keys(b0, slow ? b0 : bin_key<T>(b0), k4);
+      quad_weights(k4, even, 0, w4);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        key[i] = slow ? b + 1 - i : bin_key<T>(b + 1 - i);
-        w[i] = rw.weight(key[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (!rw.kept(key[i], w[i])) n[i] = 0;
+        key[i] = b & 2u ? k4[3 - i] : k4[1 - i];
+        w[i] = b & 2u ? w4[3 - i] : w4[1 - i];
+        if (!rw.kept(key[i])) n[i] = 0;
         if (n[i] == 0) w[i] = 0.0;
       }
     };
@@ -713,7 +747,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
         if (last >= 0) atomicMax(found, last);
         __syncthreads();
       }
-      const int g = *found;
+      const int g = min(max(*found, 0), groups - 1);
       recount(g);
       if (warp == 0) {
         uint32_t key[2], n[2];
@@ -727,14 +761,14 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
         const bool second = m1 > 0.0 && (strict ? at + m0 + m1 > limit : at + m0 + m1 >= limit);
         const uint32_t hit = __ballot_sync(0xffffffffu, first || second);
         const uint32_t any = __ballot_sync(0xffffffffu, m0 > 0.0 || m1 > 0.0);
-        // no hit: rounding inside the group, its last value that has mass
-        if (lane == (hit ? __ffs(hit) - 1 : 31 - __clz(any))) {
+        // no hit: rounding inside the group, its last value that has mass (there is one: the group's sum is not 0)
+        if (lane == (hit ? __ffs(hit) - 1 : 31 - __clz(any | 1u))) {
           const bool use0 = hit ? first : !(m1 > 0.0);
           const uint32_t cc = use0 ? n[0] : n[1];
           const double ww = use0 ? w[0] : w[1], a = use0 ? at : at + m0;
           const double q = (limit - a) / ww;
           double j = strict ? floor(q) : ceil(q) - 1.0;  // position among the equal tokens
-          j = hit ? fmin(fmax(j, 0.0), cc - 1.0) : cc - 1.0;
+          j = fmax(hit ? fmin(j, cc - 1.0) : cc - 1.0, 0.0);
           sh.key = use0 ? key[0] : key[1];
           sh.nth = static_cast<uint32_t>(j);
           sh.cum = a + (j + 1.0) * ww;
@@ -744,7 +778,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     };
 
     double kept = sh.mass[groups - 1];
-    const int k = greedy || rw.min_p > 1.0 ? 1 : sh.set_k;  // the first candidate stays whatever min_p asks
+    const int k = greedy || row_min > 1.f ? 1 : sh.set_k;  // the first candidate stays whatever min_p asks
     if (k > 0 && static_cast<uint32_t>(k) < n_all) {
       const uint32_t uk = static_cast<uint32_t>(k);
 #pragma unroll
@@ -753,7 +787,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
         if (g < groups && c[j] >= uk && (g == 0 || (j ? c[j - 1] : cb) < uk)) sh.found[0] = g;
       }
       __syncthreads();
-      const int g = sh.found[0];
+      const int g = min(sh.found[0], groups - 1);
       recount(g);
       if (warp == 0) {
         uint32_t key[2], n[2];
@@ -793,7 +827,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       }
     } else if (warp == 0) {
       // the CTA whose slice holds the nth of them: lane r asks CTA r
-      const uint32_t b = key_bin<T>(key);
+      const uint32_t b = min(key_bin<T>(key), kBins - 1u);
       uint32_t n = lane < csize ? peer(hist, lane)[b] : 0u;
       // the leader's holds everybody's
       const uint32_t others = __reduce_add_sync(0xffffffffu, lane ? n : 0u);
