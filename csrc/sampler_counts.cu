@@ -170,7 +170,7 @@ struct CountShared {
   uint32_t group_cnt[64];                     // slow path: tokens of a group's values
   int found[3];                               // the searches' groups (top-k, top-p, draw)
   double log_sum;                             // leader: log of the sum of exp(x - max)
-  uint32_t key, nth;                          // its value and rank among the value's tokens
+  uint32_t key, nth;                          // its value and rank among the value's tokens; before: of the last candidate
   double cum;                                 // mass up to and with that token
   int nth_here;                               // rank of the drawn token within this CTA's slice, or -1
   float logprob;
@@ -356,7 +356,11 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
   cluster_arrive_relaxed();
   clear();
   if (tid < 3) sh.found[tid] = kCntGroups;
-  if (tid == 0) sh.nth_here = -1;
+  if (tid == 0) {
+    sh.nth_here = -1;
+    sh.key = 0u;  // no cut
+    sh.nth = ~0u;
+  }
   if (tid == 192) {  // the row's settings, out of the registers while the slice is counted
     sh.set_t = temperature[row];
     sh.set_u = u[row];
@@ -727,7 +731,8 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
       });
       __syncthreads();
     };
-    // The first position whose cumulative mass reaches (strict: exceeds) `limit` -> sh.key, sh.nth, sh.cum.
+    // The first position whose cumulative mass reaches (strict: exceeds) `limit`, but none behind the last candidate of
+    // the cut before, whose mass was added up in another order -> sh.key, sh.nth, sh.cum.
     auto find_mass = [&](int* found, double limit, bool strict) {
       int mine = kCntGroups, last = -1;
 #pragma unroll
@@ -769,8 +774,11 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
           const double q = (limit - a) / ww;
           double j = strict ? floor(q) : ceil(q) - 1.0;  // position among the equal tokens
           j = fmax(hit ? fmin(j, cc - 1.0) : cc - 1.0, 0.0);
-          sh.key = use0 ? key[0] : key[1];
-          sh.nth = static_cast<uint32_t>(j);
+          const uint32_t kk = use0 ? key[0] : key[1], jj = static_cast<uint32_t>(j);
+          if (kk > sh.key || (kk == sh.key && jj < sh.nth)) {
+            sh.key = kk;
+            sh.nth = jj;
+          }
           sh.cum = a + (j + 1.0) * ww;
         }
       }
@@ -802,6 +810,10 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) sh.cum = (g ? sh.mass[g - 1] : 0.0) + s;
+        if (take > 0u && before + mine >= uk) {  // the k-th
+          sh.key = take > take0 ? key[1] : key[0];
+          sh.nth = (take > take0 ? take - take0 : take0) - 1u;
+        }
       }
       __syncthreads();
       kept = sh.cum;

@@ -53,3 +53,24 @@ def test_weights_a_rounding_below_min_p(device, dtype):
             x = base[r : r + 1, r:].expand(8, -1)
             check_border(x, u[:8].contiguous(), t[:8].contiguous(), m[:8].contiguous())
             check_border(x, u[40:48].contiguous(), t[40:48].contiguous(), m[40:48].contiguous())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,v", [(16, 3001), (3, 30011)])
+def test_numbers_from_one_on_take_the_last_candidate(device, dtype, rows, v):
+    """u >= 1 counts as the largest number below 1, so it names the last token that the cuts leave, in every order of
+    adding up the weights before it (each candidate holds at least 1e-7 of the mass, far above a rounding)."""
+    x, _, _ = make(rows, v, device, dtype, seed=v)
+    x[1] = x[1].abs()  # few groups of values
+    x[2, ::3] = x[2, 0]
+    off = full(rows, 1.0, device)
+    for uu in (1.0, float("inf")):
+        u = full(rows, uu, device)
+        for k in (1, 7, 50, 333):
+            kk = full(rows, k, device, torch.int32)
+            check(x, u, off, kk)
+            check(x, u, full(rows, 0.7, device), kk, full(rows, 0.9, device))
+        for p in (0.05, 0.5, 0.95):
+            check(x, u, off, None, full(rows, p, device))
+            check(x, u, off, None, full(rows, p, device), full(rows, 0.001, device))
