@@ -185,8 +185,8 @@ class GenerationEngine:
         self.quantization = quantization
         # the 8-bit copies of the projection weights, allocated before the KV cache takes the rest
         self._w8: Dict[str, ops.Int8Rows] = {}
-        self._w8_stale = quantization is not None
-        self._w8_event = None  # end of the last asynchronous copy into the weights
+        self._w8_stale = quantization is not None  # the weights changed after they were made
+        self._w8_events: List[Any] = []  # ends of the copies into the weights since then, on any stream
         if quantization is not None:
             if device.type == "cuda" and (dtype != torch.bfloat16 or cfg.hidden_size % 8 or cfg.intermediate_size % 8):
                 raise ValueError("int8 on the GPU needs bf16 and hidden and intermediate sizes that are multiples of 8")
@@ -411,16 +411,15 @@ class GenerationEngine:
             return
         if self.device.type == "cuda":
             with torch.cuda.device(self.device):
-                self._w8_event = (stream or torch.cuda.current_stream(self.device)).record_event()
+                self._w8_events.append((stream or torch.cuda.current_stream(self.device)).record_event())
         self._w8_stale = True
 
     def _refresh_int8(self) -> None:
         """Quantise the projection weights into their 8-bit copies, in place (captured graphs read them)."""
         if not self._w8_stale:
             return
-        if self._w8_event is not None:
-            torch.cuda.current_stream(self.device).wait_event(self._w8_event)
-            self._w8_event = None
+        while self._w8_events:
+            torch.cuda.current_stream(self.device).wait_event(self._w8_events.pop())
         for layer in range(self.cfg.num_hidden_layers):
             p = f"model.layers.{layer}."
             names = ["self_attn.qkv_proj.weight", "self_attn.o_proj.weight"]

@@ -1,0 +1,35 @@
+"""The engine's 8-bit copies and weights that change."""
+
+import asyncio
+
+import pytest
+import torch
+
+from accerl_agent_b200 import ops
+from accerl_agent_b200.models.transformer import build_model
+from test_engine_int8 import PROMPTS, generate_without_shutdown, make
+
+
+@pytest.mark.gpu
+def test_copies_on_several_streams_are_all_awaited():
+    """Two halves of the weights on two streams, the first behind a kernel that runs for a while, and a third update on
+    the current stream: the next step quantises none of them before they are there."""
+    cfg, m, engine = make("cuda")
+    eng = engine(quantization="int8")
+    generate_without_shutdown(eng, PROMPTS[:1], "a")
+    other = build_model(cfg, "full", torch.device("cuda"), m.params.dtype, with_grads=False)
+    other.init_weights(seed=8, std=0.08)
+    n = m.params.numel() // 2
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        torch.cuda._sleep(400_000_000)  # some 0.2 s
+    eng.load_flat_weights(other.params[:n], stream=first)
+    eng.load_flat_weights(other.params[n:], start=n, stream=second)
+    eng.load_flat_weights(other.params[-8:], start=m.params.numel() - 8)
+    generate_without_shutdown(eng, PROMPTS[:1], "b")
+    torch.cuda.synchronize()
+    for name, w in eng._w8.items():
+        expect = ops.quantize_rows(other.w(name))
+        assert torch.equal(w.q, expect.q) and torch.equal(w.scale, expect.scale), name
+    asyncio.run(eng.shutdown())
