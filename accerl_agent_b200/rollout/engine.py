@@ -187,6 +187,7 @@ class GenerationEngine:
         self._w8: Dict[str, ops.Int8Rows] = {}
         self._w8_stale = quantization is not None  # the weights changed after they were made
         self._w8_events: List[Any] = []  # ends of the copies into the weights since then, on any stream
+        self._w8_lock = threading.Lock()  # protects the two: callers note changes from any thread
         if quantization is not None:
             if device.type == "cuda" and (dtype != torch.bfloat16 or cfg.hidden_size % 8 or cfg.intermediate_size % 8):
                 raise ValueError("int8 on the GPU needs bf16 and hidden and intermediate sizes that are multiples of 8")
@@ -409,17 +410,32 @@ class GenerationEngine:
         that write ``model.params`` themselves call it afterwards."""
         if self.quantization is None:
             return
+        events = []
         if self.device.type == "cuda":
             with torch.cuda.device(self.device):
-                self._w8_events.append((stream or torch.cuda.current_stream(self.device)).record_event())
-        self._w8_stale = True
+                events.append((stream or torch.cuda.current_stream(self.device)).record_event())
+        with self._w8_lock:
+            self._w8_events += events
+            self._w8_stale = True
 
     def _refresh_int8(self) -> None:
         """Quantise the projection weights into their 8-bit copies, in place (captured graphs read them)."""
         if not self._w8_stale:
             return
-        while self._w8_events:
-            torch.cuda.current_stream(self.device).wait_event(self._w8_events.pop())
+        with self._w8_lock:  # a change that comes from here on asks for the next refresh
+            events, self._w8_events = self._w8_events, []
+            self._w8_stale = False
+        try:
+            for event in events:
+                torch.cuda.current_stream(self.device).wait_event(event)
+            self._quantize_weights()
+        except BaseException:
+            with self._w8_lock:
+                self._w8_events += events
+                self._w8_stale = True
+            raise
+
+    def _quantize_weights(self) -> None:
         for layer in range(self.cfg.num_hidden_layers):
             p = f"model.layers.{layer}."
             names = ["self_attn.qkv_proj.weight", "self_attn.o_proj.weight"]
@@ -427,7 +443,6 @@ class GenerationEngine:
                 names += ["mlp.gate_up_proj.weight", "mlp.down_proj.weight"]
             for name in names:
                 self._w8[p + name] = ops.quantize_rows(self.model.w(p + name), out=self._w8.get(p + name))
-        self._w8_stale = False
 
     def load_flat_weights(self, src: torch.Tensor, start: int = 0, stream=None) -> None:
         """Copy a fused-layout flat weight range (from a trainer, possibly a peer GPU's memory)."""

@@ -33,3 +33,39 @@ def test_copies_on_several_streams_are_all_awaited():
         expect = ops.quantize_rows(other.w(name))
         assert torch.equal(w.q, expect.q) and torch.equal(w.scale, expect.scale), name
     asyncio.run(eng.shutdown())
+
+
+def test_a_change_during_the_quantising_is_not_lost(monkeypatch):
+    """``weights_changed`` from another thread while the 8-bit copies are being made: they are made once more."""
+    cfg, m, engine = make("cpu")
+    eng = engine(quantization="int8")
+    real, calls = ops.quantize_rows, []
+
+    def quantize(x, out=None):
+        r = real(x, out=out)
+        calls.append(1)
+        if len(calls) == 1:  # the copy just made is already old
+            m.params.mul_(1.5)
+            eng.weights_changed()
+        return r
+
+    monkeypatch.setattr(ops, "quantize_rows", quantize)
+    eng.weights_changed()
+    generate_without_shutdown(eng, PROMPTS[:1], "a")
+    for name, w in eng._w8.items():
+        assert torch.equal(w.scale, real(m.w(name)).scale), name
+    # a refresh that fails is tried again
+    eng.weights_changed()
+
+    def fail(x, out=None):
+        raise RuntimeError("no")
+
+    monkeypatch.setattr(ops, "quantize_rows", fail)
+    with pytest.raises(RuntimeError):
+        eng._refresh_int8()
+    m.params.mul_(2.0)
+    monkeypatch.setattr(ops, "quantize_rows", real)
+    eng._refresh_int8()
+    for name, w in eng._w8.items():
+        assert torch.equal(w.scale, real(m.w(name)).scale), name
+    asyncio.run(eng.shutdown())
