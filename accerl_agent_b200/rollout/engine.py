@@ -39,7 +39,7 @@ import threading
 import time
 from collections import deque
 from dataclasses import dataclass, field
-from typing import Any, Deque, Dict, List, Optional
+from typing import Any, Deque, Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -840,7 +840,7 @@ class GenerationEngine:
     _BUCKETS = (8, 16, 32, 64, 128, 256, 512)
 
     def _decode_core(self, ids_d, pos_d, slots_d, table_d, lens_d, temps_d, seeds_d, offs_d, splits: int,
-                     rowslot_d=None):
+                     rowslot_d=None, top_k=None, top_p=None):
         """Forward of single-token rows (every row samples): returns (tokens, logprobs, logits) on device.
         Rows whose id is negative read their input token from the slot table (``rowslot_d``), and the
         sampled tokens are written back into it."""
@@ -857,13 +857,15 @@ class GenerationEngine:
         x = self._forward_layers(x, pos_d, slots_d, attn_fn)
         hN, _ = ops.rmsnorm(x, m.w("model.norm.weight"), cfg.rms_norm_eps)
         logits = ops.linear(hN, m.w(m.lm_head_name))
-        tok, lp = ops.sample(logits, temps_d, seeds_d, offs_d)
+        tok, lp = ops.sample(logits, temps_d, seeds_d, offs_d, top_k=top_k, top_p=top_p)
         if rowslot_d is not None:
             self._slot_tok.index_copy_(0, rowslot_d, tok)
         return tok, lp, logits
 
-    def _graph_for(self, bucket: int, width: int, keep_logits: bool = False):
-        key = (bucket, width, keep_logits)
+    def _graph_for(self, bucket: int, width: int, keep_logits: bool = False, filtered: bool = False):
+        """The captured step for ``bucket`` rows of ``width`` blocks. ``filtered``: with top-k and top-p per row (batches
+        without either leave out the sampler's third kernel)."""
+        key = (bucket, width, keep_logits, filtered)
         g = self._graphs.get(key)
         if g is not None:
             return g
@@ -888,10 +890,12 @@ class GenerationEngine:
         meta[6 * bucket :] = self.scratch_block
         splits = self.decode_splits or _decode_splits(bucket * self.cfg.num_key_value_heads)
         offs = torch.zeros(bucket, dtype=torch.int64, device=dev)
+        top_k = torch.zeros(bucket, dtype=torch.int32, device=dev) if filtered else None
+        top_p = torch.ones(bucket, dtype=torch.float32, device=dev) if filtered else None
 
         def run():
             ids, pos, slots, table, lens, seeds, rowslot = views()
-            return self._decode_core(ids, pos, slots, table, lens, temps, seeds, offs, splits, rowslot)
+            return self._decode_core(ids, pos, slots, table, lens, temps, seeds, offs, splits, rowslot, top_k, top_p)
 
         side = torch.cuda.Stream(dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -906,7 +910,7 @@ class GenerationEngine:
             out_tok, out_lp, logits = run()
         # only graphs whose steps hold min-p rows keep their logits; the others share that memory
         g = {"graph": graph, "meta": meta, "temps": temps, "offs": offs, "tok": out_tok, "lp": out_lp,
-             "logits": logits if keep_logits else None}
+             "logits": logits if keep_logits else None, "top_k": top_k, "top_p": top_p}
         del logits
         self._graphs[key] = g
         return g
@@ -948,20 +952,31 @@ class GenerationEngine:
         offs = np.zeros(bucket, dtype=np.int64)
         offs[:n] = np.fromiter((len(s.out) + s.pending for s, *_ in order), dtype=np.int64, count=n)
         return {"kind": "graph", "B": B, "bucket": bucket, "width": width, "host": host, "temps": temps, "offs": offs,
-                "min_p": _min_p_rows([s for s, *_ in order])}
+                "min_p": _min_p_rows([s for s, *_ in order]), "filters": _filters([s for s, *_ in order])}
 
     def _run_graph(self, meta):
-        g = self._graph_for(meta["bucket"], meta["width"], meta["min_p"] is not None)
+        filters = meta["filters"]
+        g = self._graph_for(meta["bucket"], meta["width"], meta["min_p"] is not None, filters is not None)
         n_meta = g["meta"].numel()
         bk = meta["bucket"]
-        host = np.empty(n_meta + 2 * bk, dtype=np.int64)
+        host = np.zeros(n_meta + (2 if filters is None else 3) * bk, dtype=np.int64)
         host[:n_meta] = meta["host"]
         host[n_meta : n_meta + bk] = meta["offs"]
-        host[n_meta + bk :].view(np.float32)[:bk] = meta["temps"]
+        floats = host[n_meta + bk : n_meta + 2 * bk].view(np.float32)  # temperatures, top-p
+        floats[:bk] = meta["temps"]
+        if filters is not None:
+            n = len(filters[0])
+            host[n_meta + 2 * bk :][:n] = filters[0]
+            floats[bk + n :] = 1.0
+            floats[bk : bk + n] = filters[1]
         d = self._h2d(host)
         g["meta"].copy_(d[:n_meta])
         g["offs"].copy_(d[n_meta : n_meta + bk])
-        g["temps"].copy_(d[n_meta + bk :].view(torch.float32)[:bk])
+        floats_d = d[n_meta + bk : n_meta + 2 * bk].view(torch.float32)
+        g["temps"].copy_(floats_d[:bk])
+        if filters is not None:
+            g["top_p"].copy_(floats_d[bk:])
+            g["top_k"].copy_(d[n_meta + 2 * bk :])
         g["graph"].replay()
         B = meta["B"]
         if meta["min_p"] is not None:
@@ -1054,8 +1069,7 @@ class GenerationEngine:
         meta["temps"] = np.asarray([float(sq.params.temperature) for sq, *_ in sampled], np.float32)
         meta["seeds"] = np.asarray([sq.seed for sq, *_ in sampled], np.int64)
         meta["offs"] = np.asarray([len(sq.out) + sq.pending for sq, *_ in sampled], np.int64)
-        if any(sq.params.top_p < 1.0 or (sq.params.top_k or -1) > 0 for sq, *_ in sampled):
-            meta["filter_params"] = [sq.params for sq, *_ in sampled]
+        meta["filters"] = _filters([sq for sq, *_ in sampled])
         meta["min_p"] = _min_p_rows([sq for sq, *_ in sampled])
         return meta
 
@@ -1135,10 +1149,8 @@ class GenerationEngine:
             xs = x.index_select(0, rows_d)
             hN, _ = ops.rmsnorm(xs, m.w("model.norm.weight"), cfg.rms_norm_eps)
             logits = ops.linear(hN, m.w(m.lm_head_name))
-            if "filter_params" in meta:
-                fp = meta["filter_params"]
-                top_k = torch.tensor([max(int(p.top_k or 0), 0) for p in fp], dtype=torch.int32)
-                top_p = torch.tensor([float(p.top_p) for p in fp], dtype=torch.float32)
+            if meta["filters"] is not None:
+                top_k, top_p = (torch.from_numpy(a) for a in meta["filters"])
                 tokens, lps = ops.sample(logits, temps_d, seeds_d, offs_d, top_k=top_k, top_p=top_p)
             else:
                 tokens, lps = ops.sample(logits, temps_d, seeds_d, offs_d)
@@ -1246,6 +1258,21 @@ class GenerationEngine:
         return None
 
 
+def _top_k(params) -> int:
+    """The request's top-k as the samplers take it (0: off)."""
+    return min(max(int(params.top_k or 0), 0), 2**31 - 1)
+
+
+def _filters(seqs) -> Optional[Tuple[np.ndarray, np.ndarray]]:
+    """top-k (int32) and top-p of the sampled sequences ``seqs``, off for the ones that min-p samples anew; None where
+    no other asks for either."""
+    plain = [getattr(s.params, "min_p", 0.0) <= 0.0 for s in seqs]
+    if not any(f and (s.params.top_p < 1.0 or _top_k(s.params) > 0) for f, s in zip(plain, seqs)):
+        return None
+    return (np.asarray([_top_k(s.params) if f else 0 for f, s in zip(plain, seqs)], np.int32),
+            np.asarray([float(s.params.top_p) if f else 1.0 for f, s in zip(plain, seqs)], np.float32))
+
+
 def _min_p_rows(seqs) -> Optional[Dict[str, Any]]:
     """Host inputs of the rows among the sampled sequences ``seqs`` that ask for min-p (None without any):
     row indices, top-k, and [u, temperature, top-p, min-p]."""
@@ -1256,7 +1283,7 @@ def _min_p_rows(seqs) -> Optional[Dict[str, Any]]:
     u = uniform_numbers(np.asarray([s.seed for s in picked], np.int64),
                         np.asarray([len(s.out) + s.pending for s in picked], np.int64))
     return {"rows": np.asarray(rows, np.int64),
-            "top_k": np.asarray([max(int(s.params.top_k or 0), 0) for s in picked], np.int64),
+            "top_k": np.asarray([_top_k(s.params) for s in picked], np.int64),
             "floats": np.asarray([u, [float(s.params.temperature) for s in picked],
                                   [float(s.params.top_p) for s in picked],
                                   [float(s.params.min_p) for s in picked]], np.float32)}
