@@ -84,9 +84,13 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None
 
 
 def linear_int8(qx, sx, qw, sw, bias=None, residual=None) -> torch.Tensor:
-    """fp32 ``sx sw (qx qw^T) (+ bias) (+ residual)``; the integer sum in 64-bit floats, where it is exact."""
+    """fp32 ``sx sw (qx qw^T) (+ bias) (+ residual)``; the integer sum in 64-bit floats, where it is exact. Scaled first
+    by the token, then by the channel, as the kernels do: the sum times a token's scale, up to 2^96 (larger ones are taken
+    2^64 times smaller and the result back), stays in fp32's range, the product of two scales need not."""
     acc = qx.double() @ qw.double().t()
-    y = acc.float() * (sx.unsqueeze(1) * sw.unsqueeze(0))
+    large = sx > 2.0 ** 96
+    y = (acc.float() * torch.where(large, sx * 2.0 ** -64, sx).unsqueeze(1)) * sw.unsqueeze(0)
+    y = y * torch.where(large, 2.0 ** 64, 1.0).to(y.dtype).unsqueeze(1)
     if bias is not None:
         y = y + bias.float()
     if residual is not None:
