@@ -789,6 +789,7 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
   const int64_t rows = logits.size(0);
   CHECK_CUDA(logits);
   TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf, "logits must be bf16 or fp16");
+  TORCH_CHECK_VALUE(rows <= 0x7fffffff && logits.size(1) <= 0x7ffffff0, "too many rows or too large a vocabulary");
   auto f32 = [&](const at::Tensor& t, const char* name) -> const float* {
     TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == rows,
                 std::string(name) + " must be contiguous float32 [rows]");
@@ -801,7 +802,8 @@ void sample_counts(const at::Tensor& logits, const at::Tensor& u, const at::Tens
     tk = top_k->data_ptr<int>();
   }
   CHECK_I64(out_tokens);
-  check(accerl_sample_counts(logits.data_ptr(), ld_of(logits), logits.scalar_type() == at::kHalf,
+  // a single row's or a single column's stride says nothing
+  check(accerl_sample_counts(logits.data_ptr(), rows <= 1 ? 0 : logits.stride(0), logits.scalar_type() == at::kHalf,
                              static_cast<int>(rows), static_cast<int>(logits.size(1)), f32(u, "u"),
                              f32(temperature, "temperature"), tk, top_p.has_value() ? f32(*top_p, "top_p") : nullptr,
                              min_p.has_value() ? f32(*min_p, "min_p") : nullptr,

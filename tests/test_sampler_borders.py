@@ -74,3 +74,15 @@ def test_numbers_from_one_on_take_the_last_candidate(device, dtype, rows, v):
         for p in (0.05, 0.5, 0.95):
             check(x, u, off, None, full(rows, p, device))
             check(x, u, off, None, full(rows, p, device), full(rows, 0.001, device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_one_column_of_any_stride(device):
+    base, u, _ = make(5, 12, device, torch.bfloat16)
+    x = base.t()[:, :1]  # [12, 1] with strides (1, 12)
+    assert x.stride(1) != 1
+    tok, lp = ops.sample_inverse_cdf(x, full(12, 0.5, device), full(12, 1.0, device))
+    assert not tok.any() and not lp.any()
+    one = base.t()[3:4, :1]
+    tok, lp = ops.sample_inverse_cdf(one, full(1, 0.5, device), full(1, 1.0, device))
+    assert not tok.any() and not lp.any()
