@@ -423,8 +423,7 @@ def linear_int8(x: Union[torch.Tensor, Int8Rows], w: Int8Rows, bias: Optional[to
             return native().linear_int8(x, w.q, w.scale, w.k, bias, residual, out, out_dtype, status)
         if x.k != w.k:
             raise ValueError(f"inner dimensions differ ({x.k} vs {w.k})")
-        return native().gemm_int8(x.q, x.scale, w.q, w.scale, w.k, bias, residual, out, out_dtype or torch.bfloat16,
-                                  status, False)
+        return native().gemm_int8(x.q, x.scale, w.q, w.scale, w.k, bias, residual, out, out_dtype or torch.bfloat16, status)
     if not isinstance(x, Int8Rows):
         out_dtype = out_dtype or x.dtype
         if x.dim() != 2 or x.shape[1] != w.k:

@@ -946,13 +946,14 @@ at::Tensor product_int8(const void* qx, const float* sx, int64_t M, const at::Te
 at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
                      const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
                      const c10::optional<at::Tensor>& out, const c10::optional<at::ScalarType>& out_dtype,
-                     const at::Tensor& status, bool w_early) {
+                     const at::Tensor& status) {
   const c10::cuda::OptionalCUDAGuard device_guard(at::device_of(qw));
   check_device(qx, qw), check_device(sx, qw);
   check_int8_rows(qw, sw, qw, K);
   check_int8_rows(qx, sx, qw, K);
+  // the kernel in front may have written the weight: no early loads
   return product_int8(qx.data_ptr(), sx.data_ptr<float>(), qx.size(0), qw, sw, K, bias, residual, out, out_dtype, status,
-                      w_early);
+                      false);
 }
 
 // The same from bf16 / fp16 activations: quantised first, the product launched to start behind that kernel.

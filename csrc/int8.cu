@@ -285,28 +285,25 @@ ACCERL_DEVINL void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_
                : "memory");
 }
 
-// The same for many rows (launched for SwiGLU): persistent blocks of 256 threads take 256 >> lg rows at a time out of
-// a ring of shared memory that bulk copies keep full, so that memory never waits for a row's reduction. Bound by
-// instructions more than by memory: [8192, 2 x 8960] takes 78 us of which its bytes need 56.
+// SwiGLU of many rows: persistent blocks of 256 threads take 256 >> lg rows at a time out of a ring of shared memory
+// that bulk copies keep full, so that memory never waits for a row's reduction. Bound by instructions more than by
+// memory: [8192, 2 x 8960] takes 78 us of which its bytes need 56.
 constexpr int kBulkThreads = 256;
 constexpr int kBulkMaxStages = 4;
 constexpr int kBulkSmem = 74 * 1024;  // three blocks an SM
-template <typename T, int PRE, int NC>
-__global__ void __launch_bounds__(kBulkThreads) quantize_rows_bulk_kernel(const T* __restrict__ x, long long ldx,
-                                                                          const T* __restrict__ w, float eps,
-                                                                          int8_t* __restrict__ q,
-                                                                          float* __restrict__ scale, long long rows,
-                                                                          int K, int Kp, int lg, int stages,
-                                                                          int* status) {
+template <int NC>
+__global__ void __launch_bounds__(kBulkThreads) quantize_rows_bulk_kernel(const __nv_bfloat16* __restrict__ x, long long ldx,
+                                                                        int8_t* __restrict__ q, float* __restrict__ scale,
+                                                                        long long rows, int K, int Kp, int lg, int stages,
+                                                                        int* status) {
   extern __shared__ uint4 ring[];
   __shared__ uint64_t full[kBulkMaxStages];
   __shared__ uint32_t red_u[2][8];
-  __shared__ float red_f[2][8];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = kBulkThreads >> lg;  // rows per stage
   const int in_row = threadIdx.x & ((1 << lg) - 1), slot = threadIdx.x >> lg;
-  const uint32_t row_bytes = static_cast<uint32_t>(K) * (PRE == kPreSwiglu ? 4u : 2u);
+  const uint32_t row_bytes = static_cast<uint32_t>(K) * 4u;
   const long long batches = (rows + per - 1) / per;
   uint8_t* base = reinterpret_cast<uint8_t*>(ring);
   auto load = [&](long long batch, int s) {  // one thread
@@ -337,23 +334,12 @@ __global__ void __launch_bounds__(kBulkThreads) quantize_rows_bulk_kernel(const 
       const int c = ((j << lg) + in_row) * 8;
       if (live && part.inside(j, c, K)) {
         part.v[j] = *reinterpret_cast<const uint4*>(src + c * 2);
-        if constexpr (PRE == kPreSwiglu) part.swiglu(j, *reinterpret_cast<const uint4*>(src + (K + c) * 2));
+        part.swiglu(j, *reinterpret_cast<const uint4*>(src + (K + c) * 2));
       } else {
         part.v[j] = make_uint4(0, 0, 0, 0);
       }
     }
     const int w0 = slot << (lg - 5);
-    if constexpr (PRE == kPreRmsNorm) {
-      float ss = part.sum_squares();
-      ss = warp_sum(ss);
-      if (lg > 5) {
-        if (lane == 0) red_f[buf][warp] = ss;
-        __syncthreads();
-        ss = red_f[buf][w0 + (lane & ((1 << (lg - 5)) - 1))];
-        for (int o = 1; o < (1 << (lg - 5)); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      }
-      part.normalise(w, rsqrtf(ss / static_cast<float>(K) + eps), in_row, lg, K);
-    }
     uint32_t amax = __reduce_max_sync(0xffffffffu, part.amax());
     if (lane == 0) red_u[buf][warp] = amax;
     // everyone has read the stage (and the wait ran out for all or for nobody)
@@ -369,8 +355,8 @@ __global__ void __launch_bounds__(kBulkThreads) quantize_rows_bulk_kernel(const 
     if (threadIdx.x == 0 && next < batches) load(next, s);
     amax = __reduce_max_sync(0xffffffffu, red_u[buf][w0 + (lane & ((1 << (lg - 5)) - 1))]);
     if (live) {
-      if (in_row == 0) scale[row] = row_scale<T>(amax);
-      part.template store<T>(q + row * Kp, amax, in_row, lg, Kp);
+      if (in_row == 0) scale[row] = row_scale<__nv_bfloat16>(amax);
+      part.template store<__nv_bfloat16>(q + row * Kp, amax, in_row, lg, Kp);
     }
     buf ^= 1;
     if (++s == stages) {
@@ -1229,15 +1215,15 @@ Int8Plan plan_int8(int M, int N, int K, bool store_ok, bool vec, int sms) {
   return plan;
 }
 
-template <typename T, int PRE, int NC>
-int launch_quantize_bulk(const T* x, long long ldx, const T* w, float eps, int8_t* q, float* scale, long long rows,
-                         int K, int Kp, int lg, int stages, int smem, int* status, cudaStream_t s) {
-  const cudaError_t e = smem_attr_once<quantize_rows_bulk_kernel<T, PRE, NC>>(kBulkSmem);
+template <int NC>
+int launch_quantize_bulk(const __nv_bfloat16* x, long long ldx, int8_t* q, float* scale, long long rows, int K, int Kp, int lg,
+                       int stages, int smem, int* status, cudaStream_t s) {
+  const cudaError_t e = smem_attr_once<quantize_rows_bulk_kernel<NC>>(kBulkSmem);
   if (e != cudaSuccess) return static_cast<int>(e);
   const long long batches = (rows + (kBulkThreads >> lg) - 1) / (kBulkThreads >> lg);
   const int resident = device_sm_count() * std::min(4, (224 * 1024) / (smem + 2048));
   const unsigned grid = static_cast<unsigned>(std::min<long long>(batches, resident));
-  quantize_rows_bulk_kernel<T, PRE, NC><<<grid, kBulkThreads, smem, s>>>(x, ldx, w, eps, q, scale, rows, K, Kp, lg, stages, status);
+  quantize_rows_bulk_kernel<NC><<<grid, kBulkThreads, smem, s>>>(x, ldx, q, scale, rows, K, Kp, lg, stages, status);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1261,22 +1247,20 @@ int launch_quantize(const T* x, long long ldx, const T* w, float eps, int8_t* q,
   int nc = (chunks + (1 << lg) - 1) >> lg;
   if constexpr (PRE == kPreSwiglu) {
     // The ring pays where an SM sees many rows: SwiGLU of 8960 columns took 78 us against 91 at 8192 rows, 37 against
-    // 33 at 2048. Plain rows and RMSNorm were never faster from it (8192 x 8960: 42 us either way; 16384 x 4096
-    // RMSNorm: 60 against 49).
+    // 33 at 2048. A ring for plain rows and RMSNorm was never faster (8192 x 8960: 42 us either way; 16384 x 4096
+    // RMSNorm: 60 against 49), and they have none.
     const int per = kBulkThreads >> lg;
     const int stage = per * K * 4;
     const int stages = std::min(kBulkMaxStages, kBulkSmem / stage);
-    if (rows > 24ll * per * device_sm_count() && nc <= 8 && stages >= 2) {
+    if (rows > 24ll * per * device_sm_count() && stages >= 2) {  // two rows of K fit: K <= 9472, at most 5 chunks
       auto launch = [&](auto n) {
-        return launch_quantize_bulk<T, PRE, decltype(n)::value>(x, ldx, w, eps, q, scale, rows, K, Kp, lg, stages,
-                                                                stages * stage, status, s);
+        return launch_quantize_bulk<decltype(n)::value>(x, ldx, q, scale, rows, K, Kp, lg, stages, stages * stage, status, s);
       };
       if (nc <= 1) return launch(std::integral_constant<int, 1>());
       if (nc <= 2) return launch(std::integral_constant<int, 2>());
       if (nc <= 3) return launch(std::integral_constant<int, 3>());
       if (nc <= 4) return launch(std::integral_constant<int, 4>());
-      if (nc <= 5) return launch(std::integral_constant<int, 5>());
-      return launch(std::integral_constant<int, 8>());
+      return launch(std::integral_constant<int, 5>());
     }
   }
   if (nc > 4) {
