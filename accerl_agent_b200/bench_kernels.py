@@ -292,7 +292,8 @@ def bench_int8(results):
         t8 = median_ms(lambda: ops.linear_int8(x, w8))
         t16 = median_ms(lambda: ops.linear(x, w))
         flops, nbytes = 2.0 * M * N * K, 2 * M * K + N * K + 2 * M * N
-        results[f"int8/{M}x{K}x{N}"] = {"ms": t8, "tops": flops / t8 / 1e9, "gbs": nbytes / t8 / 1e6, "bf16_ms": t16,
+        bt, splits = ops._native_module().int8_plan(M, N, K, N % 8 == 0, N % 4 == 0)
+        results[f"int8/{M}x{K}x{N}"] = {"kernel": f"stream {bt} tokens x {splits}" if bt else "pairs", "ms": t8, "tops": flops / t8 / 1e9, "gbs": nbytes / t8 / 1e6, "bf16_ms": t16,
                                         "floor_ms": max(flops / (2 * peak_tf) / 1e9, nbytes / peak_gbs / 1e6)}
         del x, w, w8
     for rows, V in ((1, 151936), (64, 151936), (256, 151936)):

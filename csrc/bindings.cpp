@@ -128,6 +128,7 @@ int accerl_sample_counts(const void* logits, long long ld, int half, int rows, i
                          long long* tokens, float* logprobs, cudaStream_t s);
 int accerl_quantize_rows(const void* x, long long ldx, int half, int pre, const void* w, float eps, void* q,
                          float* scale, long long rows, int K, int* status, cudaStream_t s);
+int accerl_int8_plan(int M, int N, int K, int store_ok, int vec, int* splits);
 int accerl_gemm_int8(const void* qx, const float* sx, const void* qw, const float* sw, int M, int N, int K,
                      const void* bias, const void* residual, long long ldr, int in_type, void* out, long long ldo,
                      int out_type, int w_early, int* status, cudaStream_t stream);
@@ -956,6 +957,13 @@ at::Tensor gemm_int8(const at::Tensor& qx, const at::Tensor& sx, const at::Tenso
                       false);
 }
 
+// (tokens per tile, CTAs per tile) of the streaming kernel, (0, 1): the persistent pairs
+std::tuple<int64_t, int64_t> int8_plan(int64_t M, int64_t N, int64_t K, bool store_ok, bool vec) {
+  int splits = 1;
+  const int bt = accerl_int8_plan(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), store_ok, vec, &splits);
+  return {bt, splits};
+}
+
 // The same from bf16 / fp16 activations: quantised first, the product launched to start behind that kernel.
 at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& qw, const at::Tensor& sw, int64_t K,
                        const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
@@ -1097,6 +1105,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample_counts", &sample_counts, "one token per row from given uniform numbers");
   m.def("quantize_rows", &quantize_rows, "rows to int8 with a scale each, optionally behind RMSNorm or SwiGLU");
   m.def("gemm_int8", &gemm_int8, "tcgen05 int8 GEMM with token and channel scales");
+  m.def("int8_plan", &int8_plan, "which kernel and tile gemm_int8 takes");
   m.def("linear_int8", &linear_int8, "rows to int8 and their product");
   m.def("enable_peer_access", &enable_peer_access);
   m.def("rs_sumsq", &rs_sumsq);

@@ -1303,6 +1303,14 @@ extern "C" int accerl_quantize_rows(const void* x, long long ldx, int half, int 
   return launch_quantize<__nv_bfloat16, kPreNone>(xb, ldx, nullptr, eps, qp, scale, rows, K, Kp, status, s);
 }
 
+// The kernel that accerl_gemm_int8 takes on the current device: tokens per tile of the streaming kernel and its CTAs per
+// tile, or 0 and 1 for the persistent pairs. `store_ok`, `vec`: as for plan_int8.
+extern "C" int accerl_int8_plan(int M, int N, int K, int store_ok, int vec, int* splits) {
+  const accerl::Int8Plan plan = accerl::plan_int8(M, N, K, store_ok != 0, vec != 0, accerl::device_sm_count());
+  *splits = plan.splits;
+  return plan.bt;
+}
+
 // out [M, N] (out_type) = sx sw (qx qw^T) (+ bias [N]) (+ residual [M, N]), bias and residual of in_type
 // (types: 0 bf16, 1 fp16, 2 fp32). qx [M, Kp] and qw [N, Kp], Kp = K rounded up to 16. `w_early`: the kernel
 // before this one on the stream writes nothing of the weight, so its loads need not wait for that kernel.
