@@ -71,6 +71,23 @@ class RequestOutput:
     finished: bool
 
 
+class _TurnLock:
+    """A lock that a thread which takes it again at once, as the step loop does, cannot keep from the others: whoever waits
+    for the lock holds the turn, and the loop has to wait for the turn first. (A plain lock let a pause or a weight update
+    wait for thousands of steps.)"""
+
+    def __init__(self):
+        self._turn, self._lock = threading.Lock(), threading.Lock()
+
+    def __enter__(self):
+        with self._turn:
+            self._lock.acquire()
+        return self
+
+    def __exit__(self, *exc):
+        self._lock.release()
+
+
 @dataclass
 class _Seq:
     rid: str
@@ -254,7 +271,7 @@ class GenerationEngine:
         self.paused = False
         self.version = 0  # policy version of the weights; tags every sampled token
         self._lock = threading.RLock()  # protects queues and sequence state
-        self._step_lock = threading.Lock()  # held for the duration of one engine step
+        self._step_lock = _TurnLock()  # held for the duration of one engine step
         self._wake = threading.Condition(self._lock)
         self._stop = False
         self._seed_counter = itertools.count(seed * 1_000_003 + 1)

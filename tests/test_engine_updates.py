@@ -69,3 +69,33 @@ def test_a_change_during_the_quantising_is_not_lost(monkeypatch):
     for name, w in eng._w8.items():
         assert torch.equal(w.scale, real(m.w(name)).scale), name
     asyncio.run(eng.shutdown())
+
+
+def test_a_busy_step_loop_does_not_starve_a_pause():
+    """Steps that follow each other without a break: a pause, or a weight update, gets in within a few of them."""
+    import threading
+    import time
+
+    cfg, m, engine = make("cpu")
+    eng = engine()
+    steps, stop = [0], threading.Event()
+
+    def loop():
+        while not stop.is_set():
+            with eng._step_lock:
+                steps[0] += 1
+                sum(range(20000))
+
+    t = threading.Thread(target=loop)
+    t.start()
+    try:
+        waited = []
+        for _ in range(20):
+            time.sleep(0.005)
+            before = steps[0]
+            eng.load_flat_weights(m.params)
+            waited.append(steps[0] - before)
+        assert max(waited) < 100, waited  # thousands with a plain lock
+    finally:
+        stop.set()
+        t.join()
