@@ -332,7 +332,7 @@ INT8_MAX_K = 133144  # 2^31 / 127^2: longer rows could overflow the 32-bit integ
 class Int8Rows:
     """Rows in 8-bit integers with one scale each: row ``i`` stands for ``scale[i] * q[i, :k]``.
 
-    ``q`` int8 [rows, k rounded up to 16] (zeros behind ``k``), ``scale`` fp32 [rows]. Activations (a row
+    ``q`` int8 [rows, k rounded up to 16], -127 to 127 (zeros behind ``k``), ``scale`` fp32 [rows], finite or NaN. Activations (a row
     per token) and weights (a row per output channel) are both kept this way."""
 
     q: torch.Tensor
@@ -841,7 +841,7 @@ def sample_inverse_cdf(logits: torch.Tensor, u: torch.Tensor, temperature: torch
 
     Logits of -inf and NaN are never chosen, -0 ties with 0, and +inf shares the mass with its equals. A
     row without any other logit gives token 0 with log-probability -inf. ``u`` outside [0, 1) counts as
-    the nearest number inside, NaN as 0; a NaN temperature as 0, a NaN ``top_p`` or ``min_p`` as off.
+    the nearest number inside (1 and more take the last candidate), NaN as 0; a NaN temperature as 0, a NaN ``top_p`` or ``min_p`` as off.
     Returns (tokens int64 [rows], log-probability float32 [rows] of each under softmax(logits))."""
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"logits must be [rows, V], got {tuple(logits.shape)}")

@@ -555,8 +555,8 @@ ACCERL_DEVINL void finish4(const Int8Params& p, long long t, int n, int4 acc, fl
 //   shared memory;  then all warps: a token row each, four neighbouring channels a lane (VEC: aligned rows) or
 //   every 32nd channel.
 // Bound by the latency of one CTA's chain (setup, first tile, exchange, store: about 4 us) where there are few tiles,
-// by memory where there are many. Measured without the quantising kernel: 1 x 1536 x 2048 4.9 us, 64 x 1536 x 17920
-// 11.5 us (2.6 TB/s), 256 x 8960 x 1536 14 us, 1 x 1536 x 151936 41 us (5.7 TB/s).
+// by memory where there are many. Measured without the quantising kernel: 1 x 1536 x 2048 4.7 us, 64 x 1536 x 17920
+// 11.9 us (2.5 TB/s), 256 x 8960 x 1536 14.6 us, 1 x 1536 x 151936 41 us (5.7 TB/s). VEC spills 4 bytes a thread.
 template <int OUT, bool VEC>
 __global__ void __launch_bounds__(kI8Threads) gemm_int8_stream_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                       const __grid_constant__ CUtensorMap tmX,
@@ -849,8 +849,8 @@ ACCERL_DEVINL void add_residual32(float (&f)[32], const Int8Params& p, long long
 // otherwise, and for residuals that are not aligned, through fp32 staging and coalesced element stores.
 // Bound by what L2 delivers (64 KB per 128 of K and tile: 12 to 14 TB/s in all; 5 stages, 4 cost 3 % more), where K is
 // short also by the result's way through it (8192 x 1536 x 17920: 152 us without an epilogue, 157 without its stores),
-// and by the last wave. Measured without the quantising kernel: 8192 x 1536 x
-// 17920 179 us (2.5 POP/s), 8192 x 8960 x 1536 80 us (2.8), 2048 x 4096 x 24576 143 us (2.9); 8-bit dense peak 3.3.
+// and by the last wave. Measured without the quantising kernel: 8192 x 1536 x 17920 180 us (2.5 POP/s), 8192 x 8960 x
+// 1536 85 us (2.7; 81 behind the kernel that made its rows), 2048 x 4096 x 24576 143 us (2.9); 8-bit dense peak 3.3.
 template <int OUT, bool TMA_OUT>
 __global__ void __launch_bounds__(kI8PairThreads, 1)
     gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,

@@ -8,7 +8,8 @@
 // each cut is one search for a position by count or by cumulative mass, and the draw is a last one: the first
 // position whose cumulative mass exceeds u times the mass that is left. It names a value and a rank among the
 // tokens of that value; a second look at the row (from L2) finds that token. There is no sort, one 64-bit
-// exponential per value that occurs, and only integer atomics, so a result does not depend on their order.
+// exponential per four neighbouring values (the others follow by the ratio of evenly spaced ones), and only integer
+// atomics, so a result does not depend on their order.
 //
 // Counters for all values would not fit an SM. The kernel counts a window of the values that logits take (bf16: zero
 // and 2^-40 to 2^24; fp16: below 128, each sign) in 64 KB (176 KB). Lower values, masks of the type's lowest value
@@ -24,8 +25,9 @@ namespace accerl {
 
 constexpr int kCntGroups = 1024;              // at most: groups of 64 neighbouring values
 constexpr int kCntMaxCluster = 8;
-// tokens further below the largest logit than this many temperatures weigh nothing: all of a row's together
-// hold less than 1e-20 of its mass, far below what a 64-bit sum resolves
+// tokens further below the largest logit than this many temperatures weigh nothing: each holds less than e^-60 = 9e-27
+// of the largest one's mass, all of a row's together less than 2e-17 even at 2^31 tokens (1.4e-21 at 151936), below
+// half a step of a 64-bit sum
 constexpr double kCntNegligible = 60.0;
 
 // Order-preserving 16-bit keys of the finite values and +inf: (kNegInf, kPosInf].
@@ -263,11 +265,12 @@ struct RowWeights {
 };
 
 // One row per cluster of CTAs, each counting a slice of it. Two passes over the row, the second for half of it on
-// average and from L2; between them nothing depends on V. Measured (bf16, V = 151936): 256 rows 52 us, of which the
+// average and from L2; between them nothing depends on V. Measured (bf16, V = 151936): 256 rows 53 us, of which the
 // reads need 12: shared memory adds up 32 counters at random banks in 3 to 4 clocks, so two rows on an SM, counted one
-// behind the other, take 27 us, the sums over the groups and the searches 15, the token's place 5. 1 row in 15 us, nearly
-// all of it latency (barriers of the cluster, sums of 64-bit floats, dependent searches). fp16's wider range of
-// values in use means 350 pairs of groups: 100 rows of 32003 take 26 us, 11 of them there.
+// behind the other, take 27 us, the sums over the groups and the searches 16, the token's place 5. 1 row in 16 us, nearly
+// all of it latency (barriers of the cluster, sums of 64-bit floats, dependent searches; min-p's border is 0.4 of it). fp16's wider range of
+// values in use means 350 pairs of groups: 100 rows of 32003 take 26 us, 11 of them there. An SM's 1024 threads have 64
+// registers each, a few too few: 20 bytes a thread spill (fp16: 4).
 template <typename T, int kCntThreads>
 __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
     sample_counts_kernel(const T* __restrict__ logits, long long ld, int V, const float* __restrict__ u,
@@ -639,7 +642,7 @@ __global__ void __launch_bounds__(kCntThreads, 1024 / kCntThreads)
   };
 
   if (rank == 0 && !empty) {
-    // ---- prefix sums over the groups, four a thread ----
+    // ---- prefix sums over the groups, kCntPer neighbours a thread ----
     uint32_t c[kCntPer];
     double m[kCntPer];
     uint32_t cs = 0;
