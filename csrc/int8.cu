@@ -846,7 +846,8 @@ ACCERL_DEVINL void add_residual32(float (&f)[32], const Int8Params& p, long long
 // tokens and 128 of the channels, the even CTA issues the MMAs, each drains the 128 x 256 accumulator of its
 // tokens. Accumulators are double-buffered in TMEM, so the epilogue of a tile runs under the next one's
 // products. TMA_OUT: the result leaves through swizzled shared memory and TMA stores (16-byte aligned rows);
-// otherwise, and for residuals that are not aligned, through fp32 staging and coalesced element stores.
+// otherwise (rows that end inside 16 bytes among them), and for residuals that are not aligned, through fp32 staging and
+// coalesced element stores.
 // Bound by what L2 delivers (64 KB per 128 of K and tile: 12 to 14 TB/s in all; 5 stages, 4 cost 3 % more), where K is
 // short also by the result's way through it (8192 x 1536 x 17920: 152 us without an epilogue, 157 without its stores),
 // and by the last wave. Measured without the quantising kernel: 8192 x 1536 x 17920 180 us (2.5 POP/s), 8192 x 8960 x
@@ -1338,7 +1339,9 @@ extern "C" int accerl_gemm_int8(const void* qx, const float* sx, const void* qw,
   p.status = status;
   p.w_early = w_early;
   const int es = out_type == kOutF32 ? 4 : 2, rs = in_type == kOutF32 ? 4 : 2;
+  // A TMA store cuts a row off at a multiple of 16 bytes: one that ends inside would write up to 14 bytes behind it.
   const bool store_ok = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo * es % 16 == 0 && ldo >= N &&
+                        static_cast<long long>(N) * es % 16 == 0 &&
                         (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15) == 0 && ldr * rs % 16 == 0));
   const bool vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && ldo % 4 == 0 &&
                    (reinterpret_cast<uintptr_t>(sw) & 15) == 0 &&

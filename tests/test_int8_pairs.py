@@ -108,3 +108,18 @@ def test_both_kernels_give_the_same_bits():
     for lo, hi in ((0, 1), (100, 170), (4090, 4099)):
         part = ops.linear_int8(ops.Int8Rows(r.q[lo:hi], r.scale[lo:hi], k), w, bias)
         assert torch.equal(part, whole[lo:hi])
+
+
+@pytest.mark.parametrize("dtype,n,pitch", [(torch.bfloat16, 4103, 4104), (torch.bfloat16, 4097, 4104), (torch.float16, 4100, 4104),
+                                           (torch.float32, 4101, 4104), (torch.float32, 4103, 4104), (torch.float32, 4102, 4108),
+                                           (torch.bfloat16, 143, 144)])
+def test_aligned_rows_that_end_inside_16_bytes(dtype, n, pitch):
+    """Rows that start on 16 bytes but do not end there: nothing is written behind their ends."""
+    for m, k in ((4099, 4000), (2128, 103), (70, 1536)):
+        r = ops.quantize_rows(randn(m, k, device="cuda"))
+        w = ops.quantize_rows(randn(n, k, seed=1, device="cuda", scale=0.05))
+        bias = randn(n, seed=2, device="cuda")
+        buf = torch.full((m + 1, pitch), 7.0, dtype=dtype, device="cuda")
+        out = ops.linear_int8(r, w, bias, out=buf[:m, :n])
+        check_product(out, *product64(r, w, bias))
+        assert bool((buf[m] == 7).all()) and bool((buf[:, n:] == 7).all())
