@@ -123,3 +123,28 @@ def test_aligned_rows_that_end_inside_16_bytes(dtype, n, pitch):
         out = ops.linear_int8(r, w, bias, out=buf[:m, :n])
         check_product(out, *product64(r, w, bias))
         assert bool((buf[m] == 7).all()) and bool((buf[:, n:] == 7).all())
+
+
+def test_calls_on_several_streams_at_once():
+    """Both kernels, rows behind SwiGLU and the sampler on streams of their own at the same time: the bits of the calls made
+    one after the other."""
+    k, n = 1536, 4096
+    x = randn(4099, k, device="cuda")
+    w = ops.quantize_rows(randn(n, k, seed=1, device="cuda", scale=0.05))
+    gu = randn(2048, 2 * 1544, seed=2, device="cuda", scale=2.0)
+    logits = randn(60, 50000, seed=3, device="cuda", scale=2.0)
+    u, t = torch.rand(60, device="cuda"), torch.full((60,), 0.9, device="cuda")
+    calls = [lambda: ops.linear_int8(x, w), lambda: ops.linear_int8(x[:64], w), lambda: ops.linear_int8(x[:7], w),
+             lambda: ops.swiglu_quantize(gu).q, lambda: torch.stack([a.double() for a in ops.sample_inverse_cdf(logits, u, t, top_p=t)])]
+    expect = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[] for _ in calls]
+    for _ in range(30):
+        for i, (s, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                got[i].append(c())
+    torch.cuda.synchronize()
+    for e, results in zip(expect, got):
+        assert all(torch.equal(e, r) for r in results)
+    ops.check_status(torch.device("cuda", 0))
